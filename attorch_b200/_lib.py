@@ -27,6 +27,7 @@ FLAG_WHOLE_TILES = 128
 FLAG_DROPOUT_PACKED = 256
 FLAG_DERIVATIVE_FP16 = 512
 FLAG_RESERVE_SMS_SHIFT = 16   # bits 16-23: SMs a GEMM call leaves free
+ACT_NONE = 0
 ACT_SAVED_DERIVATIVE = 22
 ACT_SAVED_DERIVATIVE_F16 = 23
 
@@ -89,6 +90,30 @@ SIGNATURES = {
     'ab200_layer_norm_workspace_bytes': (_i64, [_i64, _i64]),
     'ab200_layer_norm_backward': (_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64,
                                          _int, _int, _int, _int, _ptr, _i64, _ptr, _ptr]),
+    'ab200_grouped_linear_forward': (_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64,
+                                            _i64, _i64, _i64, _int, _int, _int, _f32, _ptr, _ptr, _int]),
+    'ab200_grouped_linear_backward_input': (_int, [_ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                                   _i64, _int, _int, _ptr, _ptr, _int]),
+    'ab200_grouped_linear_backward_weight': (_int, [_ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _int,
+                                                    _int, _ptr, _ptr, _int]),
+    'ab200_grouped_act_backward': (_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _int,
+                                          _int, _int, _f32, _ptr, _i64, _ptr]),
+    'ab200_grouped_act_backward_workspace_bytes': (_i64, [_i64, _i64, _i64]),
+    'ab200_route_forward': (_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _int,
+                                   _int, _int, _ptr, _i64, _ptr]),
+    'ab200_route_workspace_bytes': (_i64, [_i64, _i64]),
+    'ab200_route_backward': (_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _int, _int, _int,
+                                    _ptr]),
+    'ab200_expert_dispatch': (_int, [_ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _int, _ptr]),
+    'ab200_expert_combine': (_int, [_ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _int, _ptr]),
+    'ab200_expert_combine_backward': (_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64,
+                                             _i64, _int, _ptr]),
+    'ab200_float8_quantize_rows': (_int, [_ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _int, _ptr]),
+    'ab200_float8_quantize_weight': (_int, [_ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int,
+                                            _ptr]),
+    'ab200_float8_product': (_int, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64,
+                                    _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int, _int, _f32, _ptr,
+                                    _ptr, _int]),
     'ab200_multimem_all_reduce': (_int, [_ptr, _i64, _int, _int, _int, _ptr, _int, _ptr, _ptr]),
     'ab200_collective_flag_bytes': (_i64, []),
 }

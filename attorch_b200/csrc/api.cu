@@ -11,6 +11,7 @@
 #include "../../include/attorch_b200.h"
 #include "common.cuh"
 #include "gemm_launch.cuh"
+#include "grouped_launch.cuh"
 #include "kernels_misc.cuh"
 #include "act_elementwise.cuh"
 #include "glu.cuh"
@@ -159,6 +160,11 @@ int run_tiles_or_split(TcProblem& p, void* workspace, int64_t workspace_bytes, c
 }
 
 }  // namespace
+
+void count_launches(int n) { g_launches += n; }
+void set_last_path(int path) { g_last_path = path; }
+bool cta_pair_allowed(int flags) { return pair_allowed(flags); }
+
 }  // namespace ab200
 
 using namespace ab200;

@@ -1,0 +1,653 @@
+// Matrix products over ragged groups of rows (the experts of a mixture-of-experts block), sm_100a.
+//
+// Rows [offsets[e], offsets[e + 1]) of the expert-sorted activations belong to weight e of a stack:
+//
+//     forward   Y[r]  = X[r]  * W[e]      A = X   K-major,   B = W[e]  MN-major  (W[e] is [in, out])
+//     backward  dX[r] = dZ[r] * W[e]^T    A = dZ  K-major,   B = W[e]  K-major
+//     backward  dW[e] = X_e^T * dZ_e      A = X_e MN-major,  B = dZ_e  MN-major  (reduction over e's rows)
+//     8-bit     Y[r]  = X[r]  * W[e]^T    A = X   K-major,   B = W[e]  K-major   (W[e] is [out, in])
+//
+// The group boundaries are device data that the host never sees.  There is no planning launch and no
+// per-group tensor map: every CTA reads the offsets once, turns them into a prefix sum of tiles in
+// shared memory and walks its share of the tiles (worker, worker + workers, ...), so a call is one launch.
+//   * A row tile that reaches past its group's end loads rows of the next group along with its own; rows
+//     of a product are independent of each other, and the epilogue stores only the group's own.  A tile
+//     with few rows fetches only 32-row boxes that hold some.
+//   * The weights are one 3-D tensor map, so that a reduction length that is no multiple of a stage
+//     reads zeros behind a weight's last row instead of the next weight.
+//   * dW reduces over rows: a group's last k-block holds rows of the next group behind its own.  They
+//     are overwritten with zeros in shared memory (both operands: 0 * NaN is NaN) before the MMA reads
+//     the stage; that block completes on a barrier of its own, so that no other block pays for it.
+//   * Rows behind the last group (a batch with padding has fewer rows than the buffer) get zeros.
+//   * Offsets are clamped to [0, rows], made ascending and begin at 0: a bad value gives wrong rows, never a wrong
+//     address.
+// Everything else is the dense kernel's structure (gemm_tcgen05.cuh): 320 threads, one TMA producer
+// thread, one MMA issuer, 8 epilogue warps, two accumulators in tensor memory, optional CTA pairs.
+//
+// 8-bit operands (kScaled) carry one fp32 scale per row and 128 elements of K for A and per 128 x 128
+// block for B.  A stage is exactly 128 elements of K, so each stage's product is one partial sum with
+// one scale per row and 128 columns: the issuer alternates accumulators per stage, and the epilogue warps
+// add scale * partial into fp32 registers (128 accumulators a thread at BN = 256) while the next stage
+// multiplies.  Per SM a stage takes 512 clocks of MMA (128 x 256 x 128 at 8192 multiply-adds a clock)
+// against 256 clocks of tensor-memory reads and 128-256 of fp32 fma, so the scaling hides.
+#pragma once
+#include "gemm_tcgen05.cuh"
+
+namespace ab200 {
+
+constexpr int kMaxGroups = 512;
+
+struct GroupedArgs {
+  const int* offsets;     // [groups + 1] first row of every group, or NULL: one group of all rows
+  int groups;
+  int rows;               // rows of the ragged operands (some of them behind the last group)
+  int M;                  // ragged reduction: rows of each output matrix; else unused
+  int N, K;               // output columns; reduction length (ragged reduction: unused)
+  int tiles_n;            // ceil(N / BN)
+  int tiles_m;            // ragged reduction: ceil(M / TILE_M)
+  int group_m;            // row tiles per rasterisation group
+  uint32_t idesc;
+  void* out;              // [rows, N], or [groups, M, N] dense for the ragged reduction
+  long long ld_out;
+  int out_dtype;
+  void* aux;              // optional [rows, N]: pre-activation or act'(Z)
+  long long ld_aux;
+  const void* bias;       // optional [groups, N]
+  int bias_dtype;
+  int act;
+  float act_param;
+  int save_grad;
+  int grad_dtype;
+  int tma_store;          // bit 0: out, bit 1: aux
+  int* status;
+  // 8-bit operands
+  const float* a_scale;   // [K / 128][rows], pitch a_scale_ld
+  long long a_scale_ld;
+  const float* b_scale;   // + group * b_scale_group + (column / 128) * b_scale_n + (k / 128) * b_scale_k
+  long long b_scale_group, b_scale_n, b_scale_k;
+};
+
+template <int BN_, int ELT_, bool A_MN_, bool B_MN_, int CTAS_ = 1>
+struct GroupedCfg {
+  static constexpr int CTAS = CTAS_;
+  static constexpr int BM = 128;
+  static constexpr int TILE_M = BM * CTAS;
+  static constexpr int BN = BN_;
+  static constexpr int BN_CTA = BN_ / CTAS_;
+  static constexpr int ELT = ELT_;               // 1: e4m3 with block scales, 2: f16 / bf16, 4: tf32
+  static constexpr bool A_MN = A_MN_;
+  static constexpr bool B_MN = B_MN_;
+  static constexpr bool kRaggedK = A_MN_ && B_MN_;
+  static constexpr bool kScaled = ELT_ == 1;
+  static constexpr int BKE = 128 / ELT;
+  static constexpr int UMMA_K = 32 / ELT;
+  static constexpr int A_BYTES = BM * 128;
+  static constexpr int B_BYTES = BN_CTA * 128;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int kMaxSmem = 227 * 1024;
+  static constexpr int kBarrierBytes = 512;
+  static constexpr int kEpilogueWarps = 8;
+  // An epilogue warp stages 32 rows of 64 bytes for a TMA store: a 32-column chunk of a 2-byte output, half of
+  // one of an fp32 output.
+  static constexpr int kStageOutBytes = 32 * 64;
+  static constexpr int kStoreBytes = kEpilogueWarps * kStageOutBytes;
+  // Rows before each group and tiles before each group, groups + 2 entries of each.
+  static constexpr int kPlanBytes = ((2 * (kMaxGroups + 2) * 4 + 127) / 128) * 128;
+  static constexpr int kStagesFit = (kMaxSmem - 1024 - kBarrierBytes - kStoreBytes - kPlanBytes) / STAGE_BYTES;
+  static constexpr int STAGES = kStagesFit > 12 ? 12 : kStagesFit;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + kStoreBytes + kPlanBytes + 1024 + kBarrierBytes;
+  static constexpr int TMEM_COLS = (2 * BN < 32) ? 32 : 2 * BN;
+  static constexpr int MN_ATOM = 128 / ELT;
+  static constexpr int MN_BOX_BYTES = BKE * 128;
+  static constexpr bool MN_BASE32 = (ELT == 4);
+  static constexpr uint32_t MN_LAYOUT = MN_BASE32 ? ptx::kLayoutSw128Base32 : ptx::kLayoutSw128;
+  static constexpr uint32_t MN_SBO = MN_BASE32 ? 512 : 1024;
+  static constexpr int kThreads = 32 * (2 + kEpilogueWarps);
+  static constexpr int kBoxRows = 32;            // rows per box of a partly filled K-major A tile
+  static_assert(BN % 32 == 0 && BN >= 32 && BN <= 256);
+  static_assert(A_MN_ ? B_MN_ : true, "an MN-major A is the ragged reduction");
+  static_assert(!B_MN_ || BN_CTA % MN_ATOM == 0, "an MN-major B tile is made of 128-byte wide boxes");
+  static_assert(ELT_ != 1 || (!A_MN_ && !B_MN_), "8-bit operands are K-major");
+  static_assert(8 * (3 * STAGES + 4) + 8 <= kBarrierBytes);
+};
+
+// One output tile of the walk.
+struct GroupedTile {
+  int group;      // weight (ragged reduction: output matrix); -1: rows behind the last group
+  int row0;       // first output row of the tile
+  int row_end;    // end of the output rows the tile may write
+  int n_blk;
+  int k_row0;     // ragged reduction: the group's first row
+  int k_len;      // reduction length; 0: the tile is zero
+};
+
+// The plan in shared memory: first[e] = first row of group e (first[groups] = end of the last group),
+// tiles[e] = tiles before group e (tiles[groups] = before the rows behind the last group, tiles[groups + 1]
+// = all).  Built by one warp.
+template <class Cfg>
+__device__ __forceinline__ void build_plan(const GroupedArgs& a, int lane, int* first, int* tiles) {
+  int row_carry = 0, tile_carry = 0;
+  for (int base = 0; base <= a.groups; base += 32) {
+    const int e = base + lane;
+    int v = 0;
+    if (a.offsets == nullptr) v = e >= 1 ? a.rows : 0;
+    else if (e <= a.groups) v = a.offsets[e];
+    v = v < 0 ? 0 : (v > a.rows ? a.rows : v);
+    if (e == 0 || e > a.groups) v = 0;
+    v = max(v, row_carry);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xFFFFFFFFu, v, d);
+      if (lane >= d) v = max(v, up);
+    }
+    if (e <= a.groups) first[e] = v;
+    row_carry = __shfl_sync(0xFFFFFFFFu, v, 31);
+  }
+  __syncwarp();
+  for (int base = 0; base <= a.groups; base += 32) {
+    const int e = base + lane;
+    int count = 0;
+    if (e < a.groups) {
+      const int rows = first[e + 1] - first[e];
+      count = (Cfg::kRaggedK ? a.tiles_m : (rows + Cfg::TILE_M - 1) / Cfg::TILE_M) * a.tiles_n;
+    } else if (e == a.groups && !Cfg::kRaggedK) {
+      count = (a.rows - first[a.groups] + Cfg::TILE_M - 1) / Cfg::TILE_M * a.tiles_n;
+    }
+    int sum = count;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xFFFFFFFFu, sum, d);
+      if (lane >= d) sum += up;
+    }
+    if (e <= a.groups) tiles[e + 1] = tile_carry + sum;
+    tile_carry += __shfl_sync(0xFFFFFFFFu, sum, 31);
+  }
+  if (lane == 0) tiles[0] = 0;
+}
+
+template <class Cfg>
+struct GroupedIter {
+  int tile, stride;
+  __device__ __forceinline__ GroupedIter(int worker, int workers) : tile(worker), stride(workers) {}
+  __device__ __forceinline__ bool next(const GroupedArgs& a, const int* first, const int* tiles, GroupedTile& t) {
+    if (tile >= tiles[a.groups + 1]) return false;
+    int lo = 0, hi = a.groups;                        // the last e with tiles[e] <= tile
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (tiles[mid] <= tile) lo = mid;
+      else hi = mid - 1;
+    }
+    const int e = lo;
+    const int local = tile - tiles[e];
+    tile += stride;
+    int m_blk;
+    if constexpr (Cfg::kRaggedK) {
+      tile_to_blocks(local, a.tiles_m, a.tiles_n, a.group_m, m_blk, t.n_blk);
+      t.group = e;
+      t.row0 = m_blk * Cfg::TILE_M;
+      t.row_end = a.M;
+      t.k_row0 = first[e];
+      t.k_len = first[e + 1] - first[e];
+    } else {
+      const int begin = first[e];
+      const int end = e < a.groups ? first[e + 1] : a.rows;
+      tile_to_blocks(local, (end - begin + Cfg::TILE_M - 1) / Cfg::TILE_M, a.tiles_n, a.group_m, m_blk, t.n_blk);
+      t.group = e < a.groups ? e : -1;
+      t.row0 = begin + m_blk * Cfg::TILE_M;
+      t.row_end = end;
+      t.k_row0 = 0;
+      t.k_len = e < a.groups ? a.K : 0;
+    }
+    return true;
+  }
+};
+
+// This lane's 64 bytes of a 32-row chunk in the layout of a 64-byte-swizzled TMA store (16-byte unit j of row r
+// sits at unit j ^ ((r >> 1) & 3)): all 32 columns in a 2-byte type, or columns [16 part, 16 part + 16) in fp32.
+__device__ __forceinline__ void stage_row_part(uint32_t buf, int lane, int dt, int part, const float (&v)[32]) {
+  if (dt == DT_F32) {
+    const uint32_t row = buf + lane * 64;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t at = row + ((j ^ ((lane >> 1) & 3)) << 4);
+      if (part == 0)
+        ptx::st_shared_v4(at, __float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]),
+                          __float_as_uint(v[4 * j + 3]));
+      else
+        ptx::st_shared_v4(at, __float_as_uint(v[16 + 4 * j]), __float_as_uint(v[17 + 4 * j]),
+                          __float_as_uint(v[18 + 4 * j]), __float_as_uint(v[19 + 4 * j]));
+    }
+  } else {
+    stage_row_chunk(buf, lane, dt, v);
+  }
+}
+
+// Bytes of a K-major A tile that one CTA fetches for `rows` rows of it (whole 32-row boxes).
+template <class Cfg>
+__device__ __forceinline__ uint32_t a_tile_bytes(int rows) {
+  rows = rows < 0 ? 0 : (rows > Cfg::BM ? Cfg::BM : rows);
+  return static_cast<uint32_t>((rows + Cfg::kBoxRows - 1) / Cfg::kBoxRows) * (Cfg::kBoxRows * 128);
+}
+
+template <class Cfg>
+__global__ void __launch_bounds__(Cfg::kThreads, 1)
+grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a_box,
+                    const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_out,
+                    const __grid_constant__ CUtensorMap tmap_aux, const GroupedArgs args) {
+  constexpr int BM = Cfg::BM, BN = Cfg::BN, BKE = Cfg::BKE, STAGES = Cfg::STAGES;
+  constexpr int CTAS = Cfg::CTAS;
+  constexpr bool kPair = (CTAS == 2);
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = ptx::smem_u32(smem_raw);
+  const uint32_t pad = ((raw_addr + 1023u) & ~1023u) - raw_addr;
+  uint8_t* smem = smem_raw + pad;
+  const uint32_t smem_base = raw_addr + pad;
+  const uint32_t store_base = smem_base + STAGES * Cfg::STAGE_BYTES;
+  int* plan_first = reinterpret_cast<int*>(smem + STAGES * Cfg::STAGE_BYTES + Cfg::kStoreBytes);
+  int* plan_tiles = plan_first + kMaxGroups + 2;
+  uint8_t* bar_region = smem + STAGES * Cfg::STAGE_BYTES + Cfg::kStoreBytes + Cfg::kPlanBytes;
+  const uint32_t bar_base = store_base + Cfg::kStoreBytes + Cfg::kPlanBytes;
+  // Barriers (8 bytes each): full[STAGES], empty[STAGES], tail[STAGES], acc_full[2], acc_empty[2].
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
+  auto tail_bar = [&](int s) { return bar_base + 8u * (2 * STAGES + s); };
+  auto acc_full_bar = [&](int b) { return bar_base + 8u * (3 * STAGES + b); };
+  auto acc_empty_bar = [&](int b) { return bar_base + 8u * (3 * STAGES + 2 + b); };
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bar_region + 8 * (3 * STAGES + 4));
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t cta = kPair ? ptx::cluster_ctarank() : 0u;
+  const int worker = static_cast<int>(blockIdx.x) / CTAS;
+  const int workers = static_cast<int>(gridDim.x) / CTAS;
+
+  if (warp == 0 && lane == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      ptx::mbar_init(full_bar(s), 1);        // the leader's arrive.expect_tx (a zeroed tail: one plain arrival)
+      ptx::mbar_init(empty_bar(s), 1);       // one tcgen05.commit
+      ptx::mbar_init(tail_bar(s), 1);        // this CTA's arrive.expect_tx
+    }
+    for (int b = 0; b < 2; ++b) {
+      ptx::mbar_init(acc_full_bar(b), 1);
+      ptx::mbar_init(acc_empty_bar(b), Cfg::kEpilogueWarps * CTAS);
+    }
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+    ptx::prefetch_tmap(&tmap_a);
+    ptx::prefetch_tmap(&tmap_b);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc<CTAS>(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), Cfg::TMEM_COLS);
+    ptx::tmem_relinquish<CTAS>();
+  }
+  if (warp == 2) build_plan<Cfg>(args, lane, plan_first, plan_tiles);
+  ptx::tc_fence_before_sync();
+  if constexpr (kPair) {
+    ptx::cluster_arrive();
+    ptx::cluster_wait();
+  } else {
+    __syncthreads();
+  }
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+
+  auto wait = [&](uint32_t bar, uint32_t parity, int code) -> bool {
+    uint32_t spins = 0;
+    uint64_t t0 = 0;
+    while (!(kPair ? ptx::mbar_try_wait_cluster(bar, parity) : ptx::mbar_try_wait(bar, parity))) {
+      if ((++spins & 0x3FFu) == 0) {
+        if (*abort_flag) return false;
+        const uint64_t now = ptx::globaltimer_ns();
+        if (t0 == 0) {
+          t0 = now;
+        } else if (now - t0 > ptx::kWaitLimitNs) {
+          *abort_flag = 1;
+          atomicCAS(args.status, 0, code);
+          return false;
+        }
+      }
+    }
+    return true;
+  };
+
+  // The same for a whole warp: lane 0 waits, all lanes get its answer.
+  [[maybe_unused]] auto wait_warp = [&](uint32_t bar, uint32_t parity, int code) -> bool {
+    int done = 1;
+    if (lane == 0) done = wait(bar, parity, code) ? 1 : 0;
+    done = __shfl_sync(0xFFFFFFFFu, done, 0);
+    __syncwarp();
+    return done != 0;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      GroupedIter<Cfg> it(worker, workers);
+      GroupedTile t;
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      while (ok && it.next(args, plan_first, plan_tiles, t)) {
+        const int m0 = t.row0 + static_cast<int>(cta) * BM;       // this CTA's rows of A
+        const int n0 = t.n_blk * BN + static_cast<int>(cta) * Cfg::BN_CTA;
+        const int k_blocks = (t.k_len + BKE - 1) / BKE;
+        // Bytes of this CTA's and, for the leader's barrier, of the pair's loads of one stage.
+        uint32_t a_bytes = Cfg::A_BYTES, pair_a_bytes = Cfg::A_BYTES * CTAS;
+        if constexpr (!Cfg::A_MN) {
+          a_bytes = a_tile_bytes<Cfg>(t.row_end - m0);
+          pair_a_bytes = a_tile_bytes<Cfg>(t.row_end - t.row0) + (kPair ? a_tile_bytes<Cfg>(t.row_end - t.row0 - BM) : 0u);
+        }
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (!wait(empty_bar(s), ph ^ 1u, DEV_TIMEOUT_PRODUCER)) { ok = false; break; }
+          const int k0 = kb * BKE;
+          const bool tail = Cfg::kRaggedK && k0 + BKE > t.k_len;
+          uint32_t full = full_bar(s);
+          if (tail) {
+            full = tail_bar(s);
+            ptx::mbar_arrive_expect_tx(full, Cfg::STAGE_BYTES);
+            if constexpr (kPair) full = ptx::map_to_cta(full, cta);
+          } else if constexpr (kPair) {
+            if (cta == 0) ptx::mbar_arrive_expect_tx(full, pair_a_bytes + Cfg::B_BYTES * CTAS);
+            full = ptx::map_to_cta(full, 0);
+          } else {
+            ptx::mbar_arrive_expect_tx(full, a_bytes + Cfg::B_BYTES);
+          }
+          const uint32_t a_dst = smem_base + s * Cfg::STAGE_BYTES;
+          const uint32_t b_dst = a_dst + Cfg::A_BYTES;
+          if constexpr (Cfg::A_MN) {
+#pragma unroll
+            for (int j = 0; j < BM / Cfg::MN_ATOM; ++j)
+              ptx::tma_load_2d<kPair>(a_dst + j * Cfg::MN_BOX_BYTES, &tmap_a, full, m0 + j * Cfg::MN_ATOM, t.k_row0 + k0);
+          } else if (a_bytes == Cfg::A_BYTES) {
+            ptx::tma_load_2d<kPair>(a_dst, &tmap_a, full, k0, m0);
+          } else {
+            for (uint32_t off = 0; off < a_bytes; off += Cfg::kBoxRows * 128)
+              ptx::tma_load_2d<kPair>(a_dst + off, &tmap_a_box, full, k0, m0 + static_cast<int>(off / 128));
+          }
+          if constexpr (Cfg::kRaggedK) {
+#pragma unroll
+            for (int j = 0; j < Cfg::BN_CTA / Cfg::MN_ATOM; ++j)
+              ptx::tma_load_2d<kPair>(b_dst + j * Cfg::MN_BOX_BYTES, &tmap_b, full, n0 + j * Cfg::MN_ATOM, t.k_row0 + k0);
+          } else if constexpr (Cfg::B_MN) {
+#pragma unroll
+            for (int j = 0; j < Cfg::BN_CTA / Cfg::MN_ATOM; ++j)
+              ptx::tma_load_3d<kPair>(b_dst + j * Cfg::MN_BOX_BYTES, &tmap_b, full, n0 + j * Cfg::MN_ATOM, k0, t.group);
+          } else {
+            ptx::tma_load_3d<kPair>(b_dst, &tmap_b, full, k0, n0, t.group);
+          }
+          if (++s == STAGES) { s = 0; ph ^= 1u; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    // The leader's lane 0 issues.  In the ragged reduction the whole warp (of both CTAs of a pair) walks
+    // along, to clear the rows behind a group's end in its own CTA's shared memory.
+    auto issuer_wait = [&](uint32_t bar, uint32_t parity) -> bool {
+      if constexpr (Cfg::kRaggedK) return wait_warp(bar, parity, DEV_TIMEOUT_MMA);
+      else return wait(bar, parity, DEV_TIMEOUT_MMA);
+    };
+    if (Cfg::kRaggedK || (lane == 0 && cta == 0)) {
+      GroupedIter<Cfg> it(worker, workers);
+      GroupedTile t;
+      int s = 0;
+      uint32_t ph = 0;
+      uint32_t tail_ph = 0;                   // bit s: parity of tail_bar(s)
+      uint32_t n_acc = 0;
+      bool ok = true;
+      while (ok && it.next(args, plan_first, plan_tiles, t)) {
+        const int k_blocks = (t.k_len + BKE - 1) / BKE;
+        if (k_blocks == 0) continue;
+        uint32_t b = n_acc & 1u;
+        if (!Cfg::kScaled && cta == 0) {
+          if (!issuer_wait(acc_empty_bar(b), ((n_acc >> 1) & 1u) ^ 1u)) { ok = false; break; }
+          ptx::tc_fence_after_sync();
+        }
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if constexpr (Cfg::kScaled) {
+            // Every k-block is an accumulation of its own.
+            b = n_acc & 1u;
+            if (!issuer_wait(acc_empty_bar(b), ((n_acc >> 1) & 1u) ^ 1u)) { ok = false; break; }
+            ptx::tc_fence_after_sync();
+          }
+          const uint32_t a_addr = smem_base + s * Cfg::STAGE_BYTES;
+          const uint32_t b_addr = a_addr + Cfg::A_BYTES;
+          if constexpr (Cfg::kRaggedK) {
+            const int valid = t.k_len - kb * BKE;
+            if (valid < BKE) {
+              if (!issuer_wait(tail_bar(s), (tail_ph >> s) & 1u)) { ok = false; break; }
+              tail_ph ^= 1u << s;
+              // Row r of an MN-major box is its bytes [128 r, 128 r + 128), whatever the swizzle.
+              constexpr int kBoxes = (BM + Cfg::BN_CTA) / Cfg::MN_ATOM;
+              for (int j = 0; j < kBoxes; ++j)
+                for (int i = valid * 128 + lane * 16; i < Cfg::MN_BOX_BYTES; i += 512)
+                  ptx::st_shared_v4(a_addr + j * Cfg::MN_BOX_BYTES + i, 0u, 0u, 0u, 0u);
+              ptx::fence_proxy_async_smem();
+              __syncwarp();
+              if constexpr (kPair) {
+                // The leader multiplies both CTAs' operands: the other one says that its own are ready.
+                if (cta == 1) {
+                  if (lane == 0) ptx::mbar_arrive_cluster(full_bar(s), 0);
+                } else if (!issuer_wait(full_bar(s), ph)) { ok = false; break; }
+              } else if (lane == 0) {
+                ptx::mbar_arrive(full_bar(s));      // keeps the phases of the full barrier in step
+              }
+            } else if (cta == 0) {
+              if (!issuer_wait(full_bar(s), ph)) { ok = false; break; }
+            }
+          } else {
+            if (!issuer_wait(full_bar(s), ph)) { ok = false; break; }
+          }
+          ptx::tc_fence_after_sync();
+          if (lane == 0 && cta == 0) {
+            const uint32_t d_tmem = tmem_base + b * BN;
+#pragma unroll
+            for (int k = 0; k < BKE / Cfg::UMMA_K; ++k) {
+              const uint64_t a_desc =
+                  Cfg::A_MN ? ptx::make_smem_desc(a_addr + k * Cfg::UMMA_K * 128, Cfg::MN_BOX_BYTES, Cfg::MN_SBO,
+                                                  Cfg::MN_LAYOUT)
+                            : ptx::make_smem_desc(a_addr + k * 32, 16, 1024);
+              const uint64_t b_desc =
+                  Cfg::B_MN ? ptx::make_smem_desc(b_addr + k * Cfg::UMMA_K * 128, Cfg::MN_BOX_BYTES, Cfg::MN_SBO,
+                                                  Cfg::MN_LAYOUT)
+                            : ptx::make_smem_desc(b_addr + k * 32, 16, 1024);
+              const uint32_t accumulate = (k > 0 || (!Cfg::kScaled && kb > 0)) ? 1u : 0u;
+              if constexpr (Cfg::kScaled) ptx::umma_f8<CTAS>(d_tmem, a_desc, b_desc, args.idesc, accumulate);
+              else ptx::umma<CTAS, Cfg::ELT == 4>(d_tmem, a_desc, b_desc, args.idesc, accumulate);
+            }
+            if constexpr (kPair) ptx::umma_commit_pair(empty_bar(s), 3);
+            else ptx::umma_commit(empty_bar(s));
+            if (Cfg::kScaled || kb + 1 == k_blocks) {
+              if constexpr (kPair) ptx::umma_commit_pair(acc_full_bar(b), 3);
+              else ptx::umma_commit(acc_full_bar(b));
+            }
+          }
+          if (Cfg::kScaled || kb + 1 == k_blocks) ++n_acc;
+          if (++s == STAGES) { s = 0; ph ^= 1u; }
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------ epilogue (warps 2..9)
+    const int q = warp & 3;
+    const int half = (warp - 2) >> 2;
+    const uint32_t stage_buf = store_base + (warp - 2) * Cfg::kStageOutBytes;
+    constexpr int kChunks = (BN / 32 + 1) / 2;           // 32-column chunks of one epilogue warp: half, half + 2, ...
+    GroupedIter<Cfg> it(worker, workers);
+    GroupedTile t;
+    uint32_t n_acc = 0;
+    bool ok = true;
+    while (ok && it.next(args, plan_first, plan_tiles, t)) {
+      const int row0 = t.row0 + static_cast<int>(cta) * BM + q * 32;      // the warp's first row
+      const int row = row0 + lane;
+      const bool row_ok = row < t.row_end;
+      const bool rows_whole = row0 + 32 <= t.row_end || (Cfg::kRaggedK && row0 < t.row_end);
+      const int k_blocks = (t.k_len + BKE - 1) / BKE;
+      const uint32_t lane_base = static_cast<uint32_t>(q * 32) << 16;
+      [[maybe_unused]] float acc[Cfg::kScaled ? kChunks : 1][32];
+      uint32_t b = n_acc & 1u;
+
+      if constexpr (Cfg::kScaled) {
+#pragma unroll
+        for (int ci = 0; ci < kChunks; ++ci)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) acc[ci][i] = 0.0f;
+        const float* a_scale = args.a_scale + row;
+        const int nb0 = t.n_blk * BN / 128;
+        const int last_nb = (args.N - 1) / 128;
+        const float* b_scale = args.b_scale + t.group * args.b_scale_group + nb0 * args.b_scale_n;
+        const long long next_n = nb0 < last_nb ? args.b_scale_n : 0;       // second 128 columns of a 256-wide tile
+        float sa = 0.0f, sb0 = 0.0f, sb1 = 0.0f;
+        if (k_blocks > 0) {
+          sa = row_ok ? __ldg(a_scale) : 0.0f;
+          sb0 = __ldg(b_scale);
+          if (BN > 128) sb1 = __ldg(b_scale + next_n);
+        }
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          const float s0 = sa * sb0, s1 = sa * sb1;
+          if (kb + 1 < k_blocks) {
+            // The next block's scales are on their way while this one is awaited.
+            sa = row_ok ? __ldg(a_scale + (kb + 1) * args.a_scale_ld) : 0.0f;
+            sb0 = __ldg(b_scale + (kb + 1) * args.b_scale_k);
+            if (BN > 128) sb1 = __ldg(b_scale + next_n + (kb + 1) * args.b_scale_k);
+          }
+          b = n_acc & 1u;
+          if (!wait(acc_full_bar(b), (n_acc >> 1) & 1u, DEV_TIMEOUT_EPILOGUE)) { ok = false; break; }
+          ptx::tc_fence_after_sync();
+#pragma unroll
+          for (int ci = 0; ci < kChunks; ++ci) {
+            const int c = half + 2 * ci;
+            if (c < BN / 32) {
+              uint32_t r[32];
+              ptx::tmem_ld_32x32(tmem_base + lane_base + b * BN + c * 32, r);
+              ptx::tmem_ld_wait();
+              const float sc = (BN > 128 && c >= 4) ? s1 : s0;
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                const float2 f = actm::fma2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), actm::both(sc),
+                                            make_float2(acc[ci][i], acc[ci][i + 1]));
+                acc[ci][i] = f.x;
+                acc[ci][i + 1] = f.y;
+              }
+            }
+          }
+          ptx::tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (kPair) ptx::mbar_arrive_cluster(acc_empty_bar(b), 0);
+            else ptx::mbar_arrive(acc_empty_bar(b));
+          }
+          ++n_acc;
+        }
+        if (!ok) break;
+      } else if (k_blocks > 0) {
+        if (!wait(acc_full_bar(b), (n_acc >> 1) & 1u, DEV_TIMEOUT_EPILOGUE)) { ok = false; break; }
+        ptx::tc_fence_after_sync();
+      }
+
+#pragma unroll 1
+      for (int c = half; c < BN / 32; c += 2) {
+        const int col0 = t.n_blk * BN + c * 32;
+        if (col0 >= args.N || row0 >= t.row_end) break;         // warp-uniform
+        float v[32];
+        if constexpr (Cfg::kScaled) {
+          // Registers cannot be indexed at run time: a chain of selections.
+#pragma unroll
+          for (int ci = 0; ci < kChunks; ++ci)
+            if (c == half + 2 * ci) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = acc[ci][i];
+            }
+        } else if (k_blocks > 0) {
+          uint32_t r[32];
+          ptx::tmem_ld_32x32(tmem_base + lane_base + b * BN + c * 32, r);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+        }
+        const int valid = (args.N - col0 < 32) ? args.N - col0 : 32;
+        auto fused = [&]<int kOdt, int kGdt>() {
+          const int odt = kOdt >= 0 ? kOdt : args.out_dtype;
+          const int gdt = kGdt >= 0 ? kGdt : args.grad_dtype;
+          auto emit = [&](const CUtensorMap* map, void* base, long long ld, bool by_tma, const float (&w)[32], int dt) {
+            if (by_tma && rows_whole) {
+              const int parts = dt == DT_F32 ? 2 : 1;
+              for (int part = 0; part < parts; ++part) {
+                if (lane == 0) ptx::tma_store_wait_read();
+                __syncwarp();
+                stage_row_part(stage_buf, lane, dt, part, w);
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                  if constexpr (Cfg::kRaggedK) ptx::tma_store_3d(map, stage_buf, col0 + part * 16, row0, t.group);
+                  else ptx::tma_store_2d(map, stage_buf, col0 + part * 16, row0);
+                  ptx::tma_store_commit();
+                }
+              }
+            } else if (row_ok) {
+              const long long at = (Cfg::kRaggedK ? static_cast<long long>(t.group) * args.M : 0ll) + row;
+              store_row_chunk(base, dt, at * ld + col0, w, valid);
+            }
+          };
+          if (Cfg::kRaggedK || t.group < 0) {
+            emit(&tmap_out, args.out, args.ld_out, (args.tma_store & 1) != 0, v, odt);
+            if (!Cfg::kRaggedK && args.aux != nullptr) emit(&tmap_aux, args.aux, args.ld_aux, (args.tma_store & 2) != 0, v, gdt);
+            return;
+          }
+          if (args.bias != nullptr) {
+            const int elt = args.bias_dtype == DT_F32 ? 4 : 2;
+            const char* bias = static_cast<const char*>(args.bias) + static_cast<long long>(t.group) * args.N * elt;
+            add_bias_chunk(v, bias, args.bias_dtype, col0, valid, odt);
+          }
+          if (args.aux != nullptr && args.save_grad) {
+            float zr[32], g[32];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              zr[i] = v[i];
+              zr[i + 1] = v[i + 1];
+              round_through2(zr[i], zr[i + 1], odt);
+            }
+            act_fwd_grad(v, zr, g, args.act, args.act_param);
+            emit(&tmap_aux, args.aux, args.ld_aux, (args.tma_store & 2) != 0, g, gdt);
+          } else {
+            if (args.aux != nullptr) emit(&tmap_aux, args.aux, args.ld_aux, (args.tma_store & 2) != 0, v, odt);
+            act_fwd_inplace(v, args.act, args.act_param);
+          }
+          emit(&tmap_out, args.out, args.ld_out, (args.tma_store & 1) != 0, v, odt);
+        };
+        if (args.out_dtype == DT_BF16 && args.grad_dtype == DT_F16) fused.template operator()<DT_BF16, DT_F16>();
+        else fused.template operator()<-1, -1>();
+      }
+      if (!Cfg::kScaled && k_blocks > 0) {
+        ptx::tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (kPair) ptx::mbar_arrive_cluster(acc_empty_bar(b), 0);
+          else ptx::mbar_arrive(acc_empty_bar(b));
+        }
+        ++n_acc;
+      }
+    }
+    if (lane == 0) ptx::tma_store_wait_all();
+  }
+
+  ptx::tc_fence_before_sync();
+  if constexpr (kPair) {
+    ptx::cluster_arrive();
+    ptx::cluster_wait();
+  } else {
+    __syncthreads();
+  }
+  if (warp == 1) {
+    ptx::tc_fence_after_sync();
+    ptx::tmem_dealloc<CTAS>(tmem_base, Cfg::TMEM_COLS);
+  }
+}
+
+}  // namespace ab200

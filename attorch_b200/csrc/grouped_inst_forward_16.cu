@@ -1,0 +1,11 @@
+// Instantiates the grouped product (forward) for 2-byte elements.
+#include "grouped_launch.cuh"
+
+namespace ab200 {
+int launch_grouped_forward_16(const GroupedProblem& p, int bn, bool pair, cudaStream_t stream) {
+  if (pair) return launch_grouped_cfg<GroupedCfg<256, 2, false, true, 2>>(p, stream);
+  if (bn == 64) return launch_grouped_cfg<GroupedCfg<64, 2, false, true>>(p, stream);
+  if (bn == 128) return launch_grouped_cfg<GroupedCfg<128, 2, false, true>>(p, stream);
+  return launch_grouped_cfg<GroupedCfg<256, 2, false, true>>(p, stream);
+}
+}  // namespace ab200

@@ -1,0 +1,9 @@
+// Instantiates the grouped product (input) for fp32 elements, multiplied as TF32.
+#include "grouped_launch.cuh"
+
+namespace ab200 {
+int launch_grouped_input_32(const GroupedProblem& p, int bn, bool pair, cudaStream_t stream) {
+  if (pair) return launch_grouped_cfg<GroupedCfg<256, 4, false, false, 2>>(p, stream);
+  return launch_grouped_cfg<GroupedCfg<128, 4, false, false>>(p, stream);
+}
+}  // namespace ab200

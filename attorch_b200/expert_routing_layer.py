@@ -1,0 +1,345 @@
+"""
+Routing of tokens to experts and the moves between token order and expert order: ``route`` (the ``top_k``
+experts of every token, their weights, and the plan of the expert-sorted rows), ``dispatch`` (token rows to
+expert-sorted rows) and ``combine`` (expert-sorted rows to token rows, as a weighted sum), with their
+gradients; ``Router`` is the gate projection and ``route`` as a layer.
+
+No counterpart in the reference.  The device work runs in the library's kernels (``ab200_route_*``,
+``ab200_expert_*``); no value of a plan is read by the host, so nothing here synchronises.
+"""
+
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+from torch import Tensor, nn
+
+from . import _lib
+from .linear_layer import (Linear, _as_operand, _cached_size, _dtype_id, _flags_for, _ptr, _require_cuda, _stream_scratch,
+                           get_output_dtype)
+
+MAX_EXPERTS, MAX_TOP_K = 512, 32
+
+
+class Routing(NamedTuple):
+    """
+    Where every token goes.
+
+    weights:   ``[tokens, top_k]`` fp32, largest first; 0 where a token had no expert left to choose.
+    experts:   ``[tokens, top_k]`` int32, -1 where there was none.
+    offsets:   ``[num_experts + 1]`` int32: first expert-sorted row of every expert, and the end of the last.
+    row_token: ``[tokens * top_k]`` int32: the token of every row, -1 from ``offsets[-1]`` on.
+    token_row: ``[tokens, top_k]`` int32: the row of every choice, -1 where there was none.
+    """
+    weights: Tensor
+    experts: Tensor
+    offsets: Tensor
+    row_token: Tensor
+    token_row: Tensor
+
+
+def _inner_unit(tensor: Tensor) -> Tensor:
+    """The 2-D tensor itself if its rows are contiguous and do not overlap, else a contiguous copy."""
+    rows, cols = tensor.shape
+    if (cols <= 1 or tensor.stride(1) == 1) and (rows <= 1 or tensor.stride(0) >= cols):
+        return tensor
+    return tensor.contiguous()
+
+
+def _pitch(tensor: Tensor) -> int:
+    return tensor.stride(0) if tensor.shape[0] > 1 else tensor.shape[1]
+
+
+_SCORE_FUNCS = {'softmax': 0, 'sigmoid': 1}
+
+
+def _route(logits: Tensor, top_k: int, score_func: str, renormalize: bool, mask: Optional[Tensor], needs_grad: bool):
+    assert logits.ndim == 2, f'Logits must be 2D, received shape {logits.shape}'
+    tokens, experts = logits.shape
+    if score_func not in _SCORE_FUNCS:
+        raise ValueError(f"score_func must be 'softmax' or 'sigmoid', received {score_func!r}")
+    assert 1 <= experts <= MAX_EXPERTS, f'1 to {MAX_EXPERTS} experts are supported, received {experts}'
+    assert 1 <= top_k <= min(experts, MAX_TOP_K), \
+        f'top_k must be 1 to {min(experts, MAX_TOP_K)} for {experts} experts, received {top_k}'
+    _require_cuda(logits, 'logits')
+    device = logits.device
+    if mask is not None:
+        assert mask.shape == (tokens,), f'The mask must have one entry per token ({tokens}), received shape {mask.shape}'
+        assert mask.dtype is torch.bool, f'The mask must be boolean, received {mask.dtype}'
+        assert mask.device == device, f'The mask is on {mask.device}, the logits on {device}'
+        mask = mask if mask.is_contiguous() else mask.contiguous()
+    dtype = _dtype_id(logits.dtype)
+    logits = _inner_unit(logits)
+    lib = _lib.load()
+    with torch.cuda.device(device):
+        stream = torch.cuda.current_stream().cuda_stream
+        weights = torch.empty((tokens, top_k), dtype=torch.float32, device=device)
+        # Whole numbers share one allocation; the C entry takes their addresses.
+        slots = tokens * top_k
+        plan = torch.empty(3 * slots + experts + 1, dtype=torch.int32, device=device)
+        chosen, token_row, row_token, offsets = plan.split((slots, slots, slots, experts + 1))
+        stats = torch.empty((tokens, 2), dtype=torch.float32, device=device) if needs_grad else None
+        ws_bytes = _cached_size('ab200_route_workspace_bytes', tokens, experts)
+        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
+        at = plan.data_ptr()
+        _lib.check(lib.ab200_route_forward(
+            _ptr(logits), _ptr(mask), _ptr(weights), at, _ptr(stats), at + 12 * slots, at + 8 * slots, at + 4 * slots, tokens,
+            experts, top_k, _pitch(logits), dtype, _SCORE_FUNCS[score_func], int(bool(renormalize)), _ptr(workspace), ws_bytes,
+            stream), 'ab200_route_forward')
+    routing = (weights, chosen.view(tokens, top_k), offsets, row_token, token_row.view(tokens, top_k))
+    return routing, logits, stats
+
+
+class RouteAutoGrad(torch.autograd.Function):
+    """``apply(logits, top_k, score_func, renormalize, mask)`` -> the five tensors of a ``Routing``."""
+    @staticmethod
+    def forward(ctx, logits: Tensor, top_k: int, score_func: str, renormalize: bool, mask: Optional[Tensor]):
+        routing, logits, stats = _route(logits, top_k, score_func, renormalize, mask, True)
+        ctx.mark_non_differentiable(*routing[1:])
+        ctx.set_materialize_grads(False)
+        ctx.score_func, ctx.renormalize = _SCORE_FUNCS[score_func], int(bool(renormalize))
+        ctx.save_for_backward(logits, routing[0], routing[1], stats)
+        return routing
+
+    @staticmethod
+    def backward(ctx, weights_grad: Optional[Tensor], *_) -> Tuple[Optional[Tensor], ...]:
+        if weights_grad is None:
+            return None, None, None, None, None
+        logits, weights, chosen, stats = ctx.saved_tensors
+        tokens, experts = logits.shape
+        lib = _lib.load()
+        with torch.cuda.device(logits.device):
+            stream = torch.cuda.current_stream().cuda_stream
+            grad = weights_grad.float().contiguous()
+            logits_grad = torch.empty((tokens, experts), dtype=logits.dtype, device=logits.device)
+            _lib.check(lib.ab200_route_backward(
+                _ptr(logits), _ptr(weights), _ptr(chosen), _ptr(stats), _ptr(grad), _ptr(logits_grad), tokens, experts,
+                weights.shape[1], _pitch(logits), _dtype_id(logits.dtype), ctx.score_func, ctx.renormalize, stream),
+                'ab200_route_backward')
+        return logits_grad, None, None, None, None
+
+
+def route(logits: Tensor, top_k: int, score_func: str = 'softmax', renormalize: bool = True,
+          mask: Optional[Tensor] = None) -> Routing:
+    """
+    Chooses the ``top_k`` experts of every token and plans the expert-sorted rows.
+
+    Args:
+        logits: ``[tokens, num_experts]``.  The largest are chosen, equal ones by lowest index; -inf is never chosen,
+            so a token with fewer finite logits than ``top_k`` goes to fewer experts.  NaN makes a token's weights NaN.
+        top_k: Experts a token, at most 32.
+        score_func: 'softmax' (over all experts) or 'sigmoid': the weight of a chosen expert.
+        renormalize: Flag for dividing a token's weights by their sum.
+        mask: Optional ``[tokens]`` boolean; False (padding) sends a token to no expert.
+    """
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return Routing(*RouteAutoGrad.apply(logits, top_k, score_func, renormalize, mask))
+    return Routing(*_route(logits, top_k, score_func, renormalize, mask, False)[0])
+
+
+def _check_plan(routing: Routing, device: torch.device, tokens: Optional[int]) -> None:
+    assert routing.token_row.ndim == 2 and routing.token_row.dtype is torch.int32 and routing.token_row.is_contiguous() and \
+        routing.token_row.device == device, 'token_row must be a contiguous 2D int32 tensor on the device of the rows'
+    assert routing.offsets.dtype is torch.int32 and routing.offsets.is_contiguous() and routing.offsets.device == device, \
+        'offsets must be a contiguous int32 tensor on the device of the rows'
+    assert tokens is None or routing.token_row.shape[0] == tokens, \
+        f'The routing has {routing.token_row.shape[0]} tokens, the input {tokens}'
+
+
+def _row_end(routing_offsets: Tensor) -> int:
+    """Address of the end of the last expert's rows."""
+    return routing_offsets.data_ptr() + 4 * (routing_offsets.shape[0] - 1)
+
+
+def _dispatch(input: Tensor, token_row: Tensor, offsets: Tensor) -> Tensor:
+    tokens, top_k = token_row.shape
+    x = _inner_unit(input)
+    lib = _lib.load()
+    with torch.cuda.device(x.device):
+        stream = torch.cuda.current_stream().cuda_stream
+        rows = torch.empty((tokens * top_k, x.shape[1]), dtype=x.dtype, device=x.device)
+        _lib.check(lib.ab200_expert_dispatch(_ptr(x), _ptr(token_row), _row_end(offsets), _ptr(rows), tokens, top_k,
+                                             tokens * top_k, x.shape[1], _pitch(x), _dtype_id(x.dtype), stream),
+                   'ab200_expert_dispatch')
+    return rows
+
+
+def _combine(rows: Tensor, token_row: Tensor, weights: Optional[Tensor]) -> Tensor:
+    tokens, top_k = token_row.shape
+    rows = _inner_unit(rows)
+    lib = _lib.load()
+    with torch.cuda.device(rows.device):
+        stream = torch.cuda.current_stream().cuda_stream
+        output = torch.empty((tokens, rows.shape[1]), dtype=rows.dtype, device=rows.device)
+        _lib.check(lib.ab200_expert_combine(_ptr(rows), _ptr(token_row), _ptr(weights), _ptr(output), tokens, top_k,
+                                            rows.shape[0], rows.shape[1], _pitch(rows), _dtype_id(rows.dtype), stream),
+                   'ab200_expert_combine')
+    return output
+
+
+class DispatchAutoGrad(torch.autograd.Function):
+    """``apply(input, token_row, offsets)``: rows[token_row[t, j]] = input[t]."""
+    @staticmethod
+    def forward(ctx, input: Tensor, token_row: Tensor, offsets: Tensor) -> Tensor:
+        ctx.save_for_backward(token_row)
+        return _dispatch(input, token_row, offsets)
+
+    @staticmethod
+    def backward(ctx, rows_grad: Tensor) -> Tuple[Optional[Tensor], ...]:
+        token_row, = ctx.saved_tensors
+        return _combine(rows_grad, token_row, None), None, None
+
+
+class CombineAutoGrad(torch.autograd.Function):
+    """``apply(rows, weights, token_row, offsets)``: output[t] = sum_j weights[t, j] * rows[token_row[t, j]]."""
+    @staticmethod
+    def forward(ctx, rows: Tensor, weights: Tensor, token_row: Tensor, offsets: Tensor) -> Tensor:
+        ctx.needs = (rows.requires_grad, weights.requires_grad)
+        ctx.save_for_backward(rows, weights, token_row, offsets)
+        return _combine(rows, token_row, weights)
+
+    @staticmethod
+    def backward(ctx, output_grad: Tensor) -> Tuple[Optional[Tensor], ...]:
+        rows, weights, token_row, offsets = ctx.saved_tensors
+        tokens, top_k = token_row.shape
+        lib = _lib.load()
+        with torch.cuda.device(rows.device):
+            stream = torch.cuda.current_stream().cuda_stream
+            grad = _inner_unit(output_grad)
+            rows = _inner_unit(rows)
+            num_rows, dim = rows.shape
+            rows_grad = torch.empty((num_rows, dim), dtype=rows.dtype, device=rows.device) if ctx.needs[0] else None
+            weights_grad = torch.empty((tokens, top_k), dtype=torch.float32, device=rows.device) if ctx.needs[1] else None
+            _lib.check(lib.ab200_expert_combine_backward(
+                _ptr(grad), _ptr(rows), _ptr(token_row), _ptr(weights), _row_end(offsets), _ptr(rows_grad), _ptr(weights_grad),
+                tokens, top_k, num_rows, dim, _pitch(grad), _pitch(rows), _dtype_id(rows.dtype), stream),
+                'ab200_expert_combine_backward')
+        return rows_grad, weights_grad, None, None
+
+
+def dispatch(input: Tensor, routing: Routing) -> Tensor:
+    """
+    Copies every token's row to its experts: ``[tokens, dim]`` -> ``[tokens * top_k, dim]`` in expert order, zeros in
+    the rows from ``routing.offsets[-1]`` on.
+    """
+    assert input.ndim == 2, f'Inputs must be 2D, received shape {input.shape}'
+    _require_cuda(input, 'input')
+    _dtype_id(input.dtype)
+    _check_plan(routing, input.device, input.shape[0])
+    if torch.is_grad_enabled() and input.requires_grad:
+        return DispatchAutoGrad.apply(input, routing.token_row, routing.offsets)
+    return _dispatch(input, routing.token_row, routing.offsets)
+
+
+def combine(rows: Tensor, routing: Routing) -> Tensor:
+    """
+    Sums every token's expert outputs by its weights: ``[tokens * top_k, dim]`` in expert order -> ``[tokens, dim]``,
+    in fp32, rounded once.  A token without experts gets zeros.
+    """
+    assert rows.ndim == 2, f'Rows must be 2D, received shape {rows.shape}'
+    _require_cuda(rows, 'rows')
+    _dtype_id(rows.dtype)
+    _check_plan(routing, rows.device, None)
+    assert rows.shape[0] == routing.token_row.numel(), \
+        f'The routing has {routing.token_row.numel()} rows, received {rows.shape[0]}'
+    weights = routing.weights
+    assert weights.shape == routing.token_row.shape and weights.dtype is torch.float32 and weights.device == rows.device, \
+        'weights must be fp32, one per choice, on the device of the rows'
+    if not weights.is_contiguous():
+        weights = weights.contiguous()
+    if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
+        return CombineAutoGrad.apply(rows, weights, routing.token_row, routing.offsets)
+    return _combine(rows, routing.token_row, weights)
+
+
+class GateAutoGrad(torch.autograd.Function):
+    """
+    ``apply(input, weight)``: ``input @ weight`` with the bits of a row independent of timing.  ``Linear`` shares the
+    reduction of a product this narrow out over all SMs and adds the pieces atomically, in an order that changes
+    from call to call; a token whose logits nearly tie could then change its experts.  The grouped kernel with one
+    group sums every output in one place.  Backward is ``Linear``'s.
+    """
+    @staticmethod
+    def forward(ctx, input: Tensor, weight: Tensor) -> Tensor:
+        assert input.ndim == 2 and input.shape[1] == weight.shape[0], \
+            f'Incompatible input ({input.shape}) and weights ({weight.shape}) shape'
+        _require_cuda(input, 'input')
+        _require_cuda(weight, 'weight')
+        rows, in_dim = input.shape
+        experts = weight.shape[1]
+        dtype = get_output_dtype(input.dtype)
+        lib = _lib.load()
+        with torch.cuda.device(input.device):
+            stream = torch.cuda.current_stream().cuda_stream
+            x_op = _inner_unit(_as_operand(input, dtype, stream))
+            w_op = _inner_unit(_as_operand(weight, dtype, stream))
+            output = torch.empty((rows, experts), dtype=dtype, device=input.device)
+            _lib.check(lib.ab200_grouped_linear_forward(
+                _ptr(x_op), _ptr(w_op), None, None, None, _ptr(output), rows, 1, in_dim, experts, _pitch(x_op), 0, _pitch(w_op),
+                experts, experts, _dtype_id(dtype), 0, _lib.ACT_NONE, 0.0, _ptr(_stream_scratch(input.device)['status']), stream,
+                _flags_for(input.device)), 'ab200_grouped_linear_forward')
+        ctx.dtypes = (input.dtype, weight.dtype)
+        ctx.needs = (input.requires_grad, weight.requires_grad)
+        ctx.save_for_backward(x_op, w_op)
+        return output
+
+    @staticmethod
+    def backward(ctx, output_grad: Tensor) -> Tuple[Optional[Tensor], ...]:
+        x_op, w_op = ctx.saved_tensors
+        rows, in_dim = x_op.shape
+        experts, dtype, device = w_op.shape[1], x_op.dtype, x_op.device
+        lib = _lib.load()
+        input_grad = weight_grad = None
+        with torch.cuda.device(device):
+            stream = torch.cuda.current_stream().cuda_stream
+            status = _ptr(_stream_scratch(device)['status'])
+            dy = _inner_unit(_as_operand(output_grad, dtype, stream))
+            dt = _dtype_id(dtype)
+
+            def scratch(*shape: int) -> Tuple[Optional[Tensor], int]:
+                nbytes = _cached_size('ab200_gemm_workspace_bytes', *shape)
+                return (torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None), nbytes
+
+            if ctx.needs[1]:
+                weight_grad = torch.empty((in_dim, experts), dtype=ctx.dtypes[1], device=device)
+                workspace, nbytes = scratch(in_dim, experts, rows)
+                _lib.check(lib.ab200_linear_backward_weight(
+                    _ptr(x_op), _ptr(dy), _ptr(weight_grad), rows, in_dim, experts, _pitch(x_op), 1, _pitch(dy), 1, experts, dt,
+                    _dtype_id(weight_grad.dtype), _ptr(workspace), nbytes, status, stream, _flags_for(device)),
+                    'ab200_linear_backward_weight')
+            if ctx.needs[0]:
+                input_grad = torch.empty((rows, in_dim), dtype=ctx.dtypes[0], device=device)
+                workspace, nbytes = scratch(rows, in_dim, experts)
+                _lib.check(lib.ab200_linear_backward_input(
+                    _ptr(dy), _ptr(w_op), _ptr(input_grad), rows, in_dim, experts, _pitch(dy), 1, _pitch(w_op), 1, in_dim, dt,
+                    _dtype_id(input_grad.dtype), _ptr(workspace), nbytes, status, stream, _flags_for(device)),
+                    'ab200_linear_backward_input')
+        return input_grad, weight_grad
+
+
+class Router(nn.Module):
+    """
+    The gate of a mixture-of-experts block: a projection to one logit per expert, and ``route``.
+
+    Args:
+        dim: Number of input features.
+        num_experts: Number of experts, at most 512.
+        top_k: Experts a token, at most 32.
+        score_func: 'softmax' or 'sigmoid', as ``route``.
+        renormalize: Flag for dividing a token's weights by their sum.
+        device: Device to use.
+        dtype: Dtype of layer.
+    """
+    def __init__(self, dim: int, num_experts: int, top_k: int, score_func: str = 'softmax', renormalize: bool = True,
+                 device='cuda', dtype: torch.dtype = torch.float32) -> None:
+        super().__init__()
+        if not 1 <= num_experts <= MAX_EXPERTS or not 1 <= top_k <= min(num_experts, MAX_TOP_K):
+            raise RuntimeError(f'1 to {MAX_EXPERTS} experts and 1 to {MAX_TOP_K} of them a token are supported, received '
+                               f'{num_experts} and {top_k}.')
+        if score_func not in _SCORE_FUNCS:
+            raise ValueError(f"score_func must be 'softmax' or 'sigmoid', received {score_func!r}")
+        self.top_k, self.score_func, self.renormalize = top_k, score_func, renormalize
+        self.gate = Linear(dim, num_experts, bias=False, device=device, dtype=dtype)
+
+    def forward(self, input: Tensor, mask: Optional[Tensor] = None) -> Routing:
+        """``input``: ``[tokens, dim]``; ``mask``: see ``route``."""
+        return route(GateAutoGrad.apply(input, self.gate.weight), self.top_k, self.score_func, self.renormalize, mask)

@@ -1,0 +1,228 @@
+"""
+``GroupedLinear``: one ``Linear`` per group of rows (the experts of a mixture-of-experts block) as one
+layer.  ``Y[r] = act(X[r] @ W[e] + b[e])`` for the rows ``r`` in ``[offsets[e], offsets[e + 1])``; forward and
+backward (``dX``, ``dW``, ``db``) over groups of any size, none included.  ``offsets`` stays on the device: the
+group sizes are never read by the host, so a step has no synchronisation and can be captured in a CUDA graph.
+
+It has no counterpart in the reference, whose transformer block has one MLP (examples/wikitext-2/gpt.py:30-37);
+constructor, weight layout ``[in_features, out_features]`` per expert, activation strings, autocast and dtype
+rules are those of ``Linear`` (attorch/linear_layer.py:164-205).  The device work runs in the library's
+kernels (``ab200_grouped_linear_*``, ``ab200_grouped_act_backward``); there is no CPU path.
+"""
+
+import math
+from typing import Optional, Tuple
+
+import torch
+from torch import Tensor, nn
+
+from . import _lib
+from .acts import act_id, parse_act_func
+from .linear_layer import _cached_size, _dtype_id, _flags_for, _ptr, _require_cuda, _stream_scratch, get_output_dtype
+
+MAX_GROUPS = 512
+
+
+def _rows_operand(tensor: Tensor, dtype: torch.dtype, stream: int) -> Tensor:
+    """
+    A 2-D operand of ``dtype`` with unit inner stride that TMA can address where a copy can make it so:
+    the tensor itself, or a contiguous converted copy.
+    """
+    rows, cols = tensor.shape
+    elt = dtype.itemsize
+    if tensor.dtype is dtype and (cols <= 1 or tensor.stride(1) == 1):
+        pitch = tensor.stride(0) if rows > 1 else cols
+        if pitch >= cols and ((pitch * elt) % 16 == 0 and tensor.data_ptr() % 16 == 0 or (cols * elt) % 16 != 0):
+            return tensor
+    out = torch.empty((rows, cols), dtype=dtype, device=tensor.device)
+    if out.numel():
+        _lib.check(_lib.load().ab200_cast_2d(tensor.data_ptr(), out.data_ptr(), rows, cols, tensor.stride(0), tensor.stride(1),
+                                             _dtype_id(tensor.dtype), _dtype_id(dtype), stream), 'ab200_cast_2d')
+    return out
+
+
+def _pitch(tensor: Tensor) -> int:
+    """Row pitch in elements (the stride of a single row means nothing)."""
+    return tensor.stride(0) if tensor.shape[0] > 1 else tensor.shape[1]
+
+
+def _stack_operand(weight: Tensor, dtype: torch.dtype, stream: int) -> Tensor:
+    """A stack of matrices of ``dtype`` with unit inner stride and matrices a whole number of rows apart."""
+    if weight.dtype is dtype and weight.is_contiguous():
+        return weight
+    groups, rows, cols = weight.shape
+    if weight.dtype is dtype and weight.stride(2) == 1 and weight.stride(1) >= cols and \
+            weight.stride(0) >= rows * weight.stride(1) and weight.stride(0) % weight.stride(1) == 0:
+        return weight
+    flat = weight if weight.is_contiguous() else weight.contiguous()
+    if flat.dtype is dtype:
+        return flat
+    return _rows_operand(flat.view(groups * rows, cols), dtype, stream).view(groups, rows, cols)
+
+
+def _check_offsets(offsets: Tensor, groups: int, input: Tensor) -> Tensor:
+    assert offsets.ndim == 1 and offsets.shape[0] == groups + 1, \
+        f'Offsets must have one entry per group and one more ({groups + 1}), received shape {offsets.shape}'
+    assert not offsets.is_floating_point(), f'Offsets must be integers, received {offsets.dtype}'
+    _require_cuda(offsets, 'offsets')
+    assert offsets.device == input.device, f'Offsets are on {offsets.device}, the input on {input.device}'
+    return offsets if offsets.dtype is torch.int32 and offsets.is_contiguous() else offsets.int().contiguous()
+
+
+def _check_operands(input: Tensor, weight: Tensor, bias: Optional[Tensor]) -> None:
+    assert weight.ndim == 3, f'Weights must be 3D, received shape {weight.shape}'
+    assert input.ndim == 2, f'Inputs must be 2D (expert-sorted rows), received shape {input.shape}'
+    assert input.shape[1] == weight.shape[1], \
+        f'Incompatible input ({input.shape}) and weights ({weight.shape}) shape'
+    assert 1 <= weight.shape[0] <= MAX_GROUPS, f'1 to {MAX_GROUPS} groups are supported, received {weight.shape[0]}'
+    assert bias is None or bias.shape == (weight.shape[0], weight.shape[2]), \
+        f'Incompatible weights ({weight.shape}) and bias shape'
+    for name, tensor in (('input', input), ('weight', weight), ('bias', bias)):
+        if tensor is not None:
+            _require_cuda(tensor, name)
+            assert tensor.device == input.device, f'{name} is on {tensor.device}, the input on {input.device}'
+
+
+def _forward(input: Tensor, offsets: Tensor, weight: Tensor, bias: Optional[Tensor], act_func: Optional[str],
+             needs_grad: bool):
+    """(output, saved) where saved is what backward needs: operands, offsets, act'(Z)."""
+    _check_operands(input, weight, bias)
+    name, param = parse_act_func(act_func)
+    groups, in_dim, out_dim = weight.shape
+    offsets = _check_offsets(offsets, groups, input)
+    rows = input.shape[0]
+    out_dtype = get_output_dtype(input.dtype)
+    lib = _lib.load()
+    with torch.cuda.device(input.device):
+        stream = torch.cuda.current_stream().cuda_stream
+        status = _ptr(_stream_scratch(input.device)['status'])
+        x_op = _rows_operand(input, out_dtype, stream)
+        w_op = _stack_operand(weight, out_dtype, stream)
+        bias_op = bias if bias is None or bias.is_contiguous() else bias.contiguous()
+        output = torch.empty((rows, out_dim), dtype=out_dtype, device=input.device)
+        slope = None
+        flags = _flags_for(input.device)
+        if needs_grad and name is not None:
+            # act'(Z) instead of Z, in a bf16 layer as fp16, as Linear keeps it.
+            fp16 = out_dtype is torch.bfloat16
+            slope = torch.empty((rows, out_dim), dtype=torch.float16 if fp16 else out_dtype, device=input.device)
+            flags |= _lib.FLAG_SAVE_DERIVATIVE | (_lib.FLAG_DERIVATIVE_FP16 if fp16 else 0)
+        _lib.check(lib.ab200_grouped_linear_forward(
+            _ptr(x_op), _ptr(w_op), _ptr(bias_op), _ptr(offsets), _ptr(slope), _ptr(output), rows, groups, in_dim, out_dim,
+            _pitch(x_op), w_op.stride(0), w_op.stride(1), out_dim, out_dim, _dtype_id(out_dtype),
+            _dtype_id(bias_op.dtype) if bias_op is not None else 0, act_id(name), 0.0 if param is None else param, status,
+            stream, flags), 'ab200_grouped_linear_forward')
+    return output, (x_op, w_op, offsets, slope), act_id(name)
+
+
+class GroupedLinearAutoGrad(torch.autograd.Function):
+    """``apply(input, offsets, weight, bias, act_func)``: the function behind ``GroupedLinear``."""
+    @staticmethod
+    def forward(ctx, input: Tensor, offsets: Tensor, weight: Tensor, bias: Optional[Tensor] = None,
+                act_func: Optional[str] = None) -> Tensor:
+        ctx.needs = (input.requires_grad, weight.requires_grad, bias is not None and bias.requires_grad)
+        output, saved, ctx.act = _forward(input, offsets, weight, bias, act_func, any(ctx.needs))
+        ctx.dtypes = (input.dtype, weight.dtype, None if bias is None else bias.dtype)
+        if any(ctx.needs):
+            ctx.save_for_backward(*saved)
+        return output
+
+    @staticmethod
+    def backward(ctx, output_grad: Tensor) -> Tuple[Optional[Tensor], ...]:
+        x_op, w_op, offsets, slope = ctx.saved_tensors
+        groups, in_dim, out_dim = w_op.shape
+        rows, device, dtype = x_op.shape[0], x_op.device, x_op.dtype
+        dt = _dtype_id(dtype)
+        lib = _lib.load()
+        input_grad = weight_grad = bias_grad = None
+        with torch.cuda.device(device):
+            stream = torch.cuda.current_stream().cuda_stream
+            status = _ptr(_stream_scratch(device)['status'])
+            flags = _flags_for(device)
+            dy = _rows_operand(output_grad, dtype, stream)
+            dz = dy
+            if slope is not None or ctx.needs[2]:
+                if slope is not None:
+                    dz = torch.empty((rows, out_dim), dtype=dtype, device=device)
+                ws_bytes = 0
+                workspace = None
+                if ctx.needs[2]:
+                    bias_grad = torch.empty((groups, out_dim), dtype=ctx.dtypes[2], device=device)
+                    ws_bytes = _cached_size('ab200_grouped_act_backward_workspace_bytes', rows, groups, out_dim)
+                    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+                act = _lib.ACT_NONE if slope is None else (
+                    _lib.ACT_SAVED_DERIVATIVE if slope.dtype is dtype else _lib.ACT_SAVED_DERIVATIVE_F16)
+                _lib.check(lib.ab200_grouped_act_backward(
+                    _ptr(dy), _ptr(slope), _ptr(dz) if slope is not None else None, _ptr(bias_grad), _ptr(offsets), rows, groups,
+                    out_dim, _pitch(dy), out_dim, out_dim, dt, _dtype_id(bias_grad.dtype) if bias_grad is not None else 0, act, 0.0,
+                    _ptr(workspace), ws_bytes, stream), 'ab200_grouped_act_backward')
+            if ctx.needs[1]:
+                weight_grad = torch.empty((groups, in_dim, out_dim), dtype=ctx.dtypes[1], device=device)
+                _lib.check(lib.ab200_grouped_linear_backward_weight(
+                    _ptr(x_op), _ptr(dz), _ptr(offsets), _ptr(weight_grad), rows, groups, in_dim, out_dim, _pitch(x_op), _pitch(dz),
+                    dt, _dtype_id(weight_grad.dtype), status, stream, flags), 'ab200_grouped_linear_backward_weight')
+            if ctx.needs[0]:
+                input_grad = torch.empty((rows, in_dim), dtype=ctx.dtypes[0], device=device)
+                _lib.check(lib.ab200_grouped_linear_backward_input(
+                    _ptr(dz), _ptr(w_op), _ptr(offsets), _ptr(input_grad), rows, groups, in_dim, out_dim, _pitch(dz),
+                    w_op.stride(0), w_op.stride(1), in_dim, dt, _dtype_id(input_grad.dtype), status, stream, flags),
+                    'ab200_grouped_linear_backward_input')
+        return input_grad, None, weight_grad, bias_grad, None
+
+
+def grouped_linear(input: Tensor, offsets: Tensor, weight: Tensor, bias: Optional[Tensor] = None,
+                   act_func: Optional[str] = None) -> Tensor:
+    """
+    ``act(input[r] @ weight[e] + bias[e])`` for the rows ``r`` in ``[offsets[e], offsets[e + 1])``; zeros in the rows
+    from ``offsets[-1]`` on.
+
+    Args:
+        input: Expert-sorted rows ``[rows, in_features]``.
+        offsets: First row of every group and the end of the last, ``[groups + 1]`` integers on the device,
+            ascending from 0.
+        weight: ``[groups, in_features, out_features]``.
+        bias: ``[groups, out_features]`` or None.
+        act_func: Activation, as ``Linear``.
+    """
+    if torch.is_grad_enabled() and (input.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        return GroupedLinearAutoGrad.apply(input, offsets, weight, bias, act_func)
+    return _forward(input, offsets, weight, bias, act_func, False)[0]
+
+
+class GroupedLinear(nn.Module):
+    """
+    A ``Linear`` per group of rows.
+
+    Args:
+        num_groups: Number of groups (experts), at most 512.
+        in_features: Number of input features.
+        out_features: Number of output features.
+        bias: Flag for additive bias.
+        act_func: Name of the activation to fuse, as ``Linear``.
+        device: Device to use.
+        dtype: Dtype of layer.
+    """
+    def __init__(self, num_groups: int, in_features: int, out_features: int, bias: bool = True,
+                 act_func: Optional[str] = None, device='cuda', dtype: torch.dtype = torch.float32) -> None:
+        super().__init__()
+        if not 1 <= num_groups <= MAX_GROUPS:
+            raise RuntimeError(f'1 to {MAX_GROUPS} groups are supported, received {num_groups}.')
+        parse_act_func(act_func)
+        self.num_groups, self.in_features, self.out_features, self.act_func = num_groups, in_features, out_features, act_func
+        self.weight = nn.Parameter(torch.empty(num_groups, in_features, out_features, device=device, dtype=dtype))
+        self.bias = nn.Parameter(torch.empty(num_groups, out_features, device=device, dtype=dtype)) if bias else None
+        self.reset_parameters()
+
+    def reset_parameters(self) -> None:
+        """Every expert as ``Linear`` initialises itself: uniform within 1 / sqrt(in_features)."""
+        bound = 1.0 / math.sqrt(self.in_features) if self.in_features > 0 else 0.0
+        nn.init.uniform_(self.weight, -bound, bound)
+        if self.bias is not None:
+            nn.init.uniform_(self.bias, -bound, bound)
+
+    def forward(self, input: Tensor, offsets: Tensor) -> Tensor:
+        return grouped_linear(input, offsets, self.weight, self.bias, self.act_func)
+
+    def extra_repr(self) -> str:
+        return (f'num_groups={self.num_groups}, in_features={self.in_features}, out_features={self.out_features}, '
+                f'bias={self.bias is not None}, act_func={self.act_func!r}')

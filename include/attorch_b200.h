@@ -451,6 +451,139 @@ int ab200_layer_norm_backward(const void* dy, const void* x, const float* mean, 
                               void* stream);
 
 /*
+ * ---- Mixture of experts: routing, products grouped by expert, moves between token and expert order ----
+ * No counterpart in the reference: its transformer block has one MLP (examples/wikitext-2/gpt.py:30-37, 82);
+ * these entry points are that MLP with a weight per expert.  Rows sorted by expert are "ragged": expert e has
+ * rows [offsets[e], offsets[e + 1]) of a matrix of `rows` rows, `offsets` being DEVICE data of groups + 1
+ * ints that the host never reads.  offsets[0] is taken as 0; the others are clamped to [0, rows] and made
+ * ascending, so that a wrong value gives wrong rows and never a wrong address.  Rows from
+ * offsets[groups] on belong to no expert.  groups <= 512.
+ */
+
+/*
+ * Y[r] = act(X[r] W[e] + bias[e]) for the rows r of expert e; zeros in the rows behind the last.  offsets NULL
+ * (groups = 1): one weight for all rows; unlike ab200_linear_forward, which may share a reduction out and add the
+ * pieces atomically, the result then does not depend on the order in which SMs finish.
+ *   x        [rows, K] of `dtype`, row pitch ld_x
+ *   w        stack of [K, N] (the layout of Linear's weight), pitches w_group_stride and ld_w (elements)
+ *   bias     dense [groups, N] of bias_dtype, or NULL
+ *   pre_act  [rows, N] or NULL: the value before the activation, or act'(Z) with AB200_FLAG_SAVE_DERIVATIVE
+ *            (and AB200_FLAG_DERIVATIVE_FP16), as ab200_linear_forward
+ *   out      [rows, N] of `dtype`
+ * fp32 operands are multiplied as TF32.  Operands that are not 16-byte aligned, or whose pitches are no multiples
+ * of 16 bytes, run on a CUDA-core kernel.  status is required.  flags: AB200_FLAG_FORCE_GENERIC,
+ * AB200_FLAG_FORCE_TCGEN05, AB200_FLAG_NO_PAIR, AB200_FLAG_NO_TMA_STORE, AB200_FLAG_RESERVE_SMS(n).
+ */
+int ab200_grouped_linear_forward(const void* x, const void* w, const void* bias, const int* offsets, void* pre_act, void* out,
+                                 int64_t rows, int64_t groups, int64_t K, int64_t N, int64_t ld_x, int64_t w_group_stride,
+                                 int64_t ld_w, int64_t ld_pre, int64_t ld_out, int dtype, int bias_dtype, int act,
+                                 float act_param, int* status, void* stream, int flags);
+
+/* dX[r] = dZ[r] W[e]^T; zeros in the rows behind the last expert's.  dx: [rows, K] of dx_dtype. */
+int ab200_grouped_linear_backward_input(const void* dz, const void* w, const int* offsets, void* dx, int64_t rows, int64_t groups,
+                                        int64_t K, int64_t N, int64_t ld_dz, int64_t w_group_stride, int64_t ld_w, int64_t ld_dx,
+                                        int dtype, int dx_dtype, int* status, void* stream, int flags);
+
+/* dW[e] = X_e^T dZ_e over expert e's rows (zeros for an expert without rows).  dw: dense [groups, K, N] of dw_dtype. */
+int ab200_grouped_linear_backward_weight(const void* x, const void* dz, const int* offsets, void* dw, int64_t rows, int64_t groups,
+                                         int64_t K, int64_t N, int64_t ld_x, int64_t ld_dz, int dtype, int dw_dtype, int* status,
+                                         void* stream, int flags);
+
+/*
+ * dZ = dY * act'(Z) on the rows of all experts, db[e] = sum of dZ over expert e's rows (dense [groups, N]); the
+ * grouped form of ab200_act_backward, same arguments.  Rows of dz behind the last expert's are not written.
+ * Sums are fp32 in a fixed order.
+ */
+int ab200_grouped_act_backward(const void* dy, const void* z, void* dz, void* db, const int* offsets, int64_t rows, int64_t groups,
+                               int64_t N, int64_t ld_dy, int64_t ld_z, int64_t ld_dz, int dtype, int db_dtype, int act,
+                               float act_param, void* workspace, int64_t workspace_bytes, void* stream);
+
+int64_t ab200_grouped_act_backward_workspace_bytes(int64_t rows, int64_t groups, int64_t N);
+
+/*
+ * Chooses top_k experts for every token and plans the expert-sorted rows.
+ *   logits     [tokens, experts] of `dtype`, row pitch ld.  A token takes its top_k largest logits, equal ones by
+ *              lowest index; -inf is never taken; NaN is taken first and makes the token's weights NaN
+ *   mask       [tokens] bytes, 0: the token (padding) goes to no expert; or NULL
+ *   weights    [tokens, top_k] fp32, largest first.  sigmoid = 0: softmax over the whole row; 1: 1 / (1 + exp(-logit)).
+ *              renormalize: divided by their sum over the chosen.  0 where there was nothing to choose
+ *   chosen     [tokens, top_k] expert, or -1
+ *   stats      [tokens, 2] fp32 for ab200_route_backward, or NULL
+ *   offsets    [experts + 1]: first row of every expert; rows of one expert stand in token order
+ *   row_token  [tokens * top_k]: the token of every row, -1 from offsets[experts] on
+ *   token_row  [tokens, top_k]: the row of every choice, or -1
+ *   workspace  ab200_route_workspace_bytes(tokens, experts) bytes
+ * experts <= 512, top_k <= 32.
+ */
+int ab200_route_forward(const void* logits, const void* mask, float* weights, int* chosen, float* stats, int* offsets, int* row_token,
+                        int* token_row, int64_t tokens, int64_t experts, int64_t top_k, int64_t ld, int dtype, int sigmoid,
+                        int renormalize, void* workspace, int64_t workspace_bytes, void* stream);
+
+int64_t ab200_route_workspace_bytes(int64_t tokens, int64_t experts);
+
+/* logits_grad (dense [tokens, experts] of `dtype`) from the gradient of the weights ([tokens, top_k] fp32). */
+int ab200_route_backward(const void* logits, const float* weights, const int* chosen, const float* stats, const float* weights_grad,
+                         void* logits_grad, int64_t tokens, int64_t experts, int64_t top_k, int64_t ld, int dtype, int sigmoid,
+                         int renormalize, void* stream);
+
+/*
+ * rows_out[token_row[t, j]] = x[t]; zeros in the rows from *row_end (offsets[experts]) on.  x: [tokens, dim] of
+ * `dtype`, pitch ld_x; rows_out: dense [rows, dim].  Entries of token_row outside [0, rows) are skipped.
+ */
+int ab200_expert_dispatch(const void* x, const int* token_row, const int* row_end, void* rows_out, int64_t tokens, int64_t top_k,
+                          int64_t rows, int64_t dim, int64_t ld_x, int dtype, void* stream);
+
+/*
+ * y[t] = sum_j weights[t, j] rows_in[token_row[t, j]] in fp32, j ascending, rounded once; weights NULL: the plain
+ * sum (the gradient of ab200_expert_dispatch).  y: dense [tokens, dim]; entries outside [0, rows) add nothing.
+ */
+int ab200_expert_combine(const void* rows_in, const int* token_row, const float* weights, void* y, int64_t tokens, int64_t top_k,
+                         int64_t rows, int64_t dim, int64_t ld_rows, int dtype, void* stream);
+
+/*
+ * rows_grad[token_row[t, j]] = weights[t, j] dy[t] (dense [rows, dim]; zeros from *row_end on) and
+ * weights_grad[t, j] = <dy[t], rows_in[token_row[t, j]]> (fp32); either may be NULL.
+ */
+int ab200_expert_combine_backward(const void* dy, const void* rows_in, const int* token_row, const float* weights, const int* row_end,
+                                  void* rows_grad, float* weights_grad, int64_t tokens, int64_t top_k, int64_t rows, int64_t dim,
+                                  int64_t ld_dy, int64_t ld_rows, int dtype, void* stream);
+
+/*
+ * ---- Products of e4m3 operands with one fp32 scale per block of 128 (no counterpart in the reference) ----
+ */
+
+/*
+ * q = e4m3(x / s) with s the smallest power of two that keeps a block's largest magnitude within 448: blocks of
+ * 1 x 128 elements.  x: [rows, cols] of `dtype`, pitch ld_x.  q: [rows, cols] bytes, pitch ld_q (a multiple of 16, base
+ * 16-byte aligned; bytes up to the next multiple of 8 columns are written as zeros).  scale: [ceil(cols / 128)] rows of
+ * pitch ld_scale >= rows.  A block of zeros has scale 1; one with an infinity or NaN becomes NaN.
+ */
+int ab200_float8_quantize_rows(const void* x, void* q, float* scale, int64_t rows, int64_t cols, int64_t ld_x, int64_t ld_q,
+                               int64_t ld_scale, int dtype, void* stream);
+
+/*
+ * The same over blocks of 128 x 128 of a stack of matrices [rows, cols]: as stored (q, [groups, rows, cols], pitch ld_q)
+ * and transposed (q_t, [groups, cols, rows], pitch ld_q_t); either may be NULL.  scale: dense
+ * [groups, ceil(cols / 128), ceil(rows / 128)].
+ */
+int ab200_float8_quantize_weight(const void* w, void* q, void* q_t, float* scale, int64_t groups, int64_t rows, int64_t cols,
+                                 int64_t w_group_stride, int64_t ld_w, int64_t ld_q, int64_t ld_q_t, int dtype, void* stream);
+
+/*
+ * Y[r, n] = act(sum_b x_scale[b, r] w_scale[e, n / 128, b] sum_{k in block b} x[r, k] w[e, n, k] + bias[e, n])
+ * in fp32 (blocks of 128 along K), for the rows r of expert e, zeros behind the last; offsets NULL: one weight for all rows.
+ *   x        [rows, K] e4m3, pitch ld_x;  x_scale [ceil(K / 128)] rows of pitch ld_x_scale.  Any fp32 scales are allowed
+ *   w        stack of [N, K] e4m3, pitches w_group_stride, ld_w.  Bases 16-byte aligned, pitches multiples of 16
+ *   w_scale  element (e, n block, k block) at e * w_scale_group_stride + n * w_scale_stride_n + k * w_scale_stride_k
+ *   pre_act, out  of out_dtype, as ab200_grouped_linear_forward (the same flags)
+ */
+int ab200_float8_product(const void* x, const float* x_scale, const void* w, const float* w_scale, const void* bias, const int* offsets,
+                         void* pre_act, void* out, int64_t rows, int64_t groups, int64_t K, int64_t N, int64_t ld_x, int64_t ld_x_scale,
+                         int64_t w_group_stride, int64_t ld_w, int64_t w_scale_group_stride, int64_t w_scale_stride_n,
+                         int64_t w_scale_stride_k, int64_t ld_pre, int64_t ld_out, int out_dtype, int bias_dtype, int act,
+                         float act_param, int* status, void* stream, int flags);
+
+/*
  * In-place SUM all-reduce of a gradient bucket over the GPUs of one NVSwitch domain (one process per
  * GPU), through NVLink multicast: the switch adds the ranks' copies (multimem.ld_reduce) and writes the
  * sums back to all of them (multimem.st); see csrc/allreduce_multimem.cu.  No counterpart in the
