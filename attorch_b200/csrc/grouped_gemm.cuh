@@ -21,15 +21,16 @@
 //   * Rows behind the last group (a batch with padding has fewer rows than the buffer) get zeros.
 //   * Offsets are clamped to [0, rows], made ascending and begin at 0: a bad value gives wrong rows, never a wrong
 //     address.
-// Everything else is the dense kernel's structure (gemm_tcgen05.cuh): 320 threads, one TMA producer
+// Everything else is the dense kernel's structure (gemm_tcgen05.cuh): one TMA producer
 // thread, one MMA issuer, 8 epilogue warps, two accumulators in tensor memory, optional CTA pairs.
 //
 // 8-bit operands (kScaled) carry one fp32 scale per row and 128 elements of K for A and per 128 x 128
-// block for B.  A stage is exactly 128 elements of K, so each stage's product is one partial sum with
-// one scale per row and 128 columns: the issuer alternates accumulators per stage, and the epilogue warps
-// add scale * partial into fp32 registers (128 accumulators a thread at BN = 256) while the next stage
-// multiplies.  Per SM a stage takes 512 clocks of MMA (128 x 256 x 128 at 8192 multiply-adds a clock)
-// against 256 clocks of tensor-memory reads and 128-256 of fp32 fma, so the scaling hides.
+// block for B.  A stage is exactly 128 elements of K, so each stage's product over 128 columns is one partial
+// sum with one scale per row: the issuer gives every such part one of four accumulators of 128 columns, and the
+// epilogue warps add scale * partial into fp32 registers (128 accumulators a thread at BN = 256) while the
+// next parts multiply.  Per SM a part takes 256 clocks of MMA (128 x 128 x 128 at 8192 multiply-adds a clock)
+// against 128 clocks of tensor-memory reads and 64-128 of fp32 fma, so the scaling can hide; four
+// accumulators cover the way there and back (commit, wake-up, read, arrival: about 600 clocks).
 #pragma once
 #include "gemm_tcgen05.cuh"
 
@@ -93,22 +94,38 @@ struct GroupedCfg {
   static constexpr int kStoreBytes = kEpilogueWarps * kStageOutBytes;
   // Rows before each group and tiles before each group, groups + 2 entries of each.
   static constexpr int kPlanBytes = ((2 * (kMaxGroups + 2) * 4 + 127) / 128) * 128;
-  static constexpr int kStagesFit = (kMaxSmem - 1024 - kBarrierBytes - kStoreBytes - kPlanBytes) / STAGE_BYTES;
+  // Accumulators in tensor memory: two of the tile's width, or, with scales, four of at most 128 columns (one per
+  // stage and 128-column part of the tile).
+  static constexpr int SUB = kScaled && BN > 128 ? 128 : BN;
+  static constexpr int kSubs = BN / SUB;
+  static constexpr int kAccs = kScaled ? 4 : 2;
+  static constexpr int TMEM_COLS = kAccs * SUB;
+  // Ring of scales: 128 rows' and up to two column blocks' of four k-blocks (one wait for four).
+  static constexpr int kScaleStages = 4;
+  static constexpr int kScaleBlocks = 4;
+  static constexpr int kScaleStageBytes = kScaleBlocks * (BM + 4) * 4;
+  static constexpr int kScaleBytes = kScaled ? kScaleStages * kScaleStageBytes : 0;
+  static constexpr int kStagesFit = (kMaxSmem - 1024 - kBarrierBytes - kStoreBytes - kPlanBytes - kScaleBytes) / STAGE_BYTES;
   static constexpr int STAGES = kStagesFit > 12 ? 12 : kStagesFit;
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + kStoreBytes + kPlanBytes + 1024 + kBarrierBytes;
-  static constexpr int TMEM_COLS = (2 * BN < 32) ? 32 : 2 * BN;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + kStoreBytes + kPlanBytes + kScaleBytes + 1024 + kBarrierBytes;
   static constexpr int MN_ATOM = 128 / ELT;
   static constexpr int MN_BOX_BYTES = BKE * 128;
   static constexpr bool MN_BASE32 = (ELT == 4);
   static constexpr uint32_t MN_LAYOUT = MN_BASE32 ? ptx::kLayoutSw128Base32 : ptx::kLayoutSw128;
   static constexpr uint32_t MN_SBO = MN_BASE32 ? 512 : 1024;
-  static constexpr int kThreads = 32 * (2 + kEpilogueWarps);
+  // 8-bit: 12 warps, the epilogue's two warpgroups (warps 4-11) take registers over from the first one: with
+  // 168 a thread (384 threads at launch) part of the 128 accumulators lived in local memory, and a stage took 3 us
+  // instead of 0.3.  256 * 216 + 128 * 72 = 384 * 168.
+  static constexpr int kFirstEpilogueWarp = kScaled ? 4 : 2;
+  static constexpr int kThreads = 32 * (kFirstEpilogueWarp + kEpilogueWarps);
+  static constexpr int kEpilogueRegs = 216, kOtherRegs = 72;
   static constexpr int kBoxRows = 32;            // rows per box of a partly filled K-major A tile
   static_assert(BN % 32 == 0 && BN >= 32 && BN <= 256);
   static_assert(A_MN_ ? B_MN_ : true, "an MN-major A is the ragged reduction");
   static_assert(!B_MN_ || BN_CTA % MN_ATOM == 0, "an MN-major B tile is made of 128-byte wide boxes");
   static_assert(ELT_ != 1 || (!A_MN_ && !B_MN_), "8-bit operands are K-major");
-  static_assert(8 * (3 * STAGES + 4) + 8 <= kBarrierBytes);
+  static_assert(8 * (3 * STAGES + 8 + 2 * kScaleStages) + 8 <= kBarrierBytes);
+  static_assert((TMEM_COLS & (TMEM_COLS - 1)) == 0 && TMEM_COLS >= 32 && TMEM_COLS <= 512);
 };
 
 // One output tile of the walk.
@@ -222,6 +239,47 @@ __device__ __forceinline__ void stage_row_part(uint32_t buf, int lane, int dt, i
   }
 }
 
+// Up to 8 consecutive elements of one row.
+__device__ __forceinline__ void store_slice(void* base, int dt, long long offset, const float (&v)[8], int valid) {
+  if (dt == DT_F32) {
+    float* p = static_cast<float*>(base) + offset;
+    if (valid >= 8 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+      reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+      return;
+    }
+  } else {
+    uint16_t* p = static_cast<uint16_t*>(base) + offset;
+    if (valid >= 8 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+      *reinterpret_cast<uint4*>(p) = make_uint4(pack2(v[0], v[1], dt), pack2(v[2], v[3], dt), pack2(v[4], v[5], dt), pack2(v[6], v[7], dt));
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < valid) store_from_f32(base, dt, offset + i, v[i]);
+}
+
+// act_fwd_grad over 8 elements at a time: v <- act(v), and put(first element, act' of the 8) at v rounded to dt.
+template <class F>
+__device__ __forceinline__ void act_fwd_grad_slices(float (&v)[32], int act, float p, int dt, F&& put) {
+  dispatch_act(act, [&]<int A>() {
+#pragma unroll
+    for (int i0 = 0; i0 < 32; i0 += 8) {
+      float g[8];
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        float z0 = v[i0 + i], z1 = v[i0 + i + 1], y0, y1;
+        round_through2(z0, z1, dt);
+        actm::fwd_grad2<A>(v[i0 + i], v[i0 + i + 1], z0, z1, p, y0, y1, g[i], g[i + 1]);
+        v[i0 + i] = y0;
+        v[i0 + i + 1] = y1;
+      }
+      put(i0, g);
+    }
+  });
+}
+
 // Bytes of a K-major A tile that one CTA fetches for `rows` rows of it (whole 32-row boxes).
 template <class Cfg>
 __device__ __forceinline__ uint32_t a_tile_bytes(int rows) {
@@ -246,15 +304,21 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   const uint32_t store_base = smem_base + STAGES * Cfg::STAGE_BYTES;
   int* plan_first = reinterpret_cast<int*>(smem + STAGES * Cfg::STAGE_BYTES + Cfg::kStoreBytes);
   int* plan_tiles = plan_first + kMaxGroups + 2;
-  uint8_t* bar_region = smem + STAGES * Cfg::STAGE_BYTES + Cfg::kStoreBytes + Cfg::kPlanBytes;
-  const uint32_t bar_base = store_base + Cfg::kStoreBytes + Cfg::kPlanBytes;
-  // Barriers (8 bytes each): full[STAGES], empty[STAGES], tail[STAGES], acc_full[2], acc_empty[2].
+  const uint32_t scale_base = store_base + Cfg::kStoreBytes + Cfg::kPlanBytes;
+  [[maybe_unused]] const float* scale_ring =
+      reinterpret_cast<const float*>(smem + STAGES * Cfg::STAGE_BYTES + Cfg::kStoreBytes + Cfg::kPlanBytes);
+  uint8_t* bar_region = smem + STAGES * Cfg::STAGE_BYTES + Cfg::kStoreBytes + Cfg::kPlanBytes + Cfg::kScaleBytes;
+  const uint32_t bar_base = scale_base + Cfg::kScaleBytes;
+  // Barriers (8 bytes each): full[STAGES], empty[STAGES], tail[STAGES], acc_full[4], acc_empty[4], scale_full and
+  // scale_empty[kScaleStages].
   auto full_bar = [&](int s) { return bar_base + 8u * s; };
   auto empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
   auto tail_bar = [&](int s) { return bar_base + 8u * (2 * STAGES + s); };
   auto acc_full_bar = [&](int b) { return bar_base + 8u * (3 * STAGES + b); };
-  auto acc_empty_bar = [&](int b) { return bar_base + 8u * (3 * STAGES + 2 + b); };
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bar_region + 8 * (3 * STAGES + 4));
+  auto acc_empty_bar = [&](int b) { return bar_base + 8u * (3 * STAGES + 4 + b); };
+  auto scale_full_bar = [&](int b) { return bar_base + 8u * (3 * STAGES + 8 + b); };
+  auto scale_empty_bar = [&](int b) { return bar_base + 8u * (3 * STAGES + 8 + Cfg::kScaleStages + b); };
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bar_region + 8 * (3 * STAGES + 8 + 2 * Cfg::kScaleStages));
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const int warp = threadIdx.x >> 5;
@@ -269,10 +333,15 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       ptx::mbar_init(empty_bar(s), 1);       // one tcgen05.commit
       ptx::mbar_init(tail_bar(s), 1);        // this CTA's arrive.expect_tx
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < Cfg::kAccs; ++b) {
       ptx::mbar_init(acc_full_bar(b), 1);
       ptx::mbar_init(acc_empty_bar(b), Cfg::kEpilogueWarps * CTAS);
     }
+    if (Cfg::kScaled)
+      for (int b = 0; b < Cfg::kScaleStages; ++b) {
+        ptx::mbar_init(scale_full_bar(b), 32);                      // the copies of each lane of the scale loader
+        ptx::mbar_init(scale_empty_bar(b), Cfg::kEpilogueWarps);
+      }
     *abort_flag = 0;
     ptx::fence_mbar_init();
     ptx::prefetch_tmap(&tmap_a);
@@ -282,7 +351,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     ptx::tmem_alloc<CTAS>(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), Cfg::TMEM_COLS);
     ptx::tmem_relinquish<CTAS>();
   }
-  if (warp == 2) build_plan<Cfg>(args, lane, plan_first, plan_tiles);
+  if (warp == Cfg::kFirstEpilogueWarp) build_plan<Cfg>(args, lane, plan_first, plan_tiles);
   ptx::tc_fence_before_sync();
   if constexpr (kPair) {
     ptx::cluster_arrive();
@@ -321,6 +390,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     return done != 0;
   };
 
+  if (warp < Cfg::kFirstEpilogueWarp) {
+  // The register counts change at the top of the two branches, so that the compiler knows which holds where.
+  if constexpr (Cfg::kScaled) ptx::registers_dec<Cfg::kOtherRegs>();
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0) {
@@ -374,6 +446,12 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
 #pragma unroll
             for (int j = 0; j < Cfg::BN_CTA / Cfg::MN_ATOM; ++j)
               ptx::tma_load_3d<kPair>(b_dst + j * Cfg::MN_BOX_BYTES, &tmap_b, full, n0 + j * Cfg::MN_ATOM, k0, t.group);
+          } else if constexpr (Cfg::kSubs > 1) {
+            // Each 128-column part of the tile is a product of its own: of a pair, each CTA holds half of its columns.
+#pragma unroll
+            for (int j = 0; j < Cfg::kSubs; ++j)
+              ptx::tma_load_3d<kPair>(b_dst + j * (Cfg::SUB / CTAS) * 128, &tmap_b, full, k0,
+                                      t.n_blk * BN + j * Cfg::SUB + static_cast<int>(cta) * (Cfg::SUB / CTAS), t.group);
           } else {
             ptx::tma_load_3d<kPair>(b_dst, &tmap_b, full, k0, n0, t.group);
           }
@@ -383,13 +461,12 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
-    // The leader's lane 0 issues.  In the ragged reduction the whole warp (of both CTAs of a pair) walks
-    // along, to clear the rows behind a group's end in its own CTA's shared memory.
+    // The leader's warp walks the tiles converged and elects a lane to issue.  In the ragged reduction the other
+    // CTA's does too, to clear the rows behind a group's end in its own shared memory.
     auto issuer_wait = [&](uint32_t bar, uint32_t parity) -> bool {
-      if constexpr (Cfg::kRaggedK) return wait_warp(bar, parity, DEV_TIMEOUT_MMA);
-      else return wait(bar, parity, DEV_TIMEOUT_MMA);
+      return __all_sync(0xFFFFFFFFu, wait(bar, parity, DEV_TIMEOUT_MMA));
     };
-    if (Cfg::kRaggedK || (lane == 0 && cta == 0)) {
+    if (Cfg::kRaggedK || cta == 0) {
       GroupedIter<Cfg> it(worker, workers);
       GroupedTile t;
       int s = 0;
@@ -400,18 +477,12 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       while (ok && it.next(args, plan_first, plan_tiles, t)) {
         const int k_blocks = (t.k_len + BKE - 1) / BKE;
         if (k_blocks == 0) continue;
-        uint32_t b = n_acc & 1u;
+        const uint32_t b = n_acc & 1u;
         if (!Cfg::kScaled && cta == 0) {
           if (!issuer_wait(acc_empty_bar(b), ((n_acc >> 1) & 1u) ^ 1u)) { ok = false; break; }
           ptx::tc_fence_after_sync();
         }
         for (int kb = 0; kb < k_blocks; ++kb) {
-          if constexpr (Cfg::kScaled) {
-            // Every k-block is an accumulation of its own.
-            b = n_acc & 1u;
-            if (!issuer_wait(acc_empty_bar(b), ((n_acc >> 1) & 1u) ^ 1u)) { ok = false; break; }
-            ptx::tc_fence_after_sync();
-          }
           const uint32_t a_addr = smem_base + s * Cfg::STAGE_BYTES;
           const uint32_t b_addr = a_addr + Cfg::A_BYTES;
           if constexpr (Cfg::kRaggedK) {
@@ -441,7 +512,32 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
             if (!issuer_wait(full_bar(s), ph)) { ok = false; break; }
           }
           ptx::tc_fence_after_sync();
-          if (lane == 0 && cta == 0) {
+          if constexpr (Cfg::kScaled) {
+            // Every k-block and 128-column part of the tile is an accumulation of its own.
+#pragma unroll
+            for (int j = 0; j < Cfg::kSubs; ++j) {
+              const uint32_t d = n_acc % Cfg::kAccs;
+              if (!issuer_wait(acc_empty_bar(d), ((n_acc / Cfg::kAccs) & 1u) ^ 1u)) { ok = false; break; }
+              ptx::tc_fence_after_sync();
+              if (ptx::elect_one()) {
+#pragma unroll
+                for (int k = 0; k < BKE / Cfg::UMMA_K; ++k)
+                  ptx::umma_f8<CTAS>(tmem_base + d * Cfg::SUB, ptx::make_smem_desc(a_addr + k * 32, 16, 1024),
+                                     ptx::make_smem_desc(b_addr + j * (Cfg::SUB / CTAS) * 128 + k * 32, 16, 1024), args.idesc,
+                                     k > 0 ? 1u : 0u);
+                if constexpr (kPair) ptx::umma_commit_pair(acc_full_bar(d), 3);
+                else ptx::umma_commit(acc_full_bar(d));
+                if (j + 1 == Cfg::kSubs) {
+                  if constexpr (kPair) ptx::umma_commit_pair(empty_bar(s), 3);
+                  else ptx::umma_commit(empty_bar(s));
+                }
+              }
+              __syncwarp();
+              ++n_acc;
+            }
+            if (!ok) break;
+          } else if (cta == 0) {
+            if (ptx::elect_one()) {
             const uint32_t d_tmem = tmem_base + b * BN;
 #pragma unroll
             for (int k = 0; k < BKE / Cfg::UMMA_K; ++k) {
@@ -453,32 +549,66 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
                   Cfg::B_MN ? ptx::make_smem_desc(b_addr + k * Cfg::UMMA_K * 128, Cfg::MN_BOX_BYTES, Cfg::MN_SBO,
                                                   Cfg::MN_LAYOUT)
                             : ptx::make_smem_desc(b_addr + k * 32, 16, 1024);
-              const uint32_t accumulate = (k > 0 || (!Cfg::kScaled && kb > 0)) ? 1u : 0u;
-              if constexpr (Cfg::kScaled) ptx::umma_f8<CTAS>(d_tmem, a_desc, b_desc, args.idesc, accumulate);
-              else ptx::umma<CTAS, Cfg::ELT == 4>(d_tmem, a_desc, b_desc, args.idesc, accumulate);
+              ptx::umma<CTAS, Cfg::ELT == 4>(d_tmem, a_desc, b_desc, args.idesc, (kb > 0 || k > 0) ? 1u : 0u);
             }
             if constexpr (kPair) ptx::umma_commit_pair(empty_bar(s), 3);
             else ptx::umma_commit(empty_bar(s));
-            if (Cfg::kScaled || kb + 1 == k_blocks) {
+            if (kb + 1 == k_blocks) {
               if constexpr (kPair) ptx::umma_commit_pair(acc_full_bar(b), 3);
               else ptx::umma_commit(acc_full_bar(b));
             }
+            }
+            __syncwarp();
           }
-          if (Cfg::kScaled || kb + 1 == k_blocks) ++n_acc;
+          if (!Cfg::kScaled && kb + 1 == k_blocks) ++n_acc;
           if (++s == STAGES) { s = 0; ph ^= 1u; }
         }
       }
     }
     __syncwarp();
+  } else if (Cfg::kScaled && warp == 2) {
+    // ------------------------------------------------------------------ scale loader
+    // Runs up to 16 k-blocks ahead of the epilogue: read where they are used, the scales' latency (1000 clocks) was the
+    // time of a stage.
+    GroupedIter<Cfg> it(worker, workers);
+    GroupedTile t;
+    uint32_t n = 0;
+    bool ok = true;
+    while (ok && it.next(args, plan_first, plan_tiles, t)) {
+      const int k_blocks = (t.k_len + BKE - 1) / BKE;
+      const int row0 = t.row0 + static_cast<int>(cta) * BM;
+      const float* a_scale = args.a_scale + row0;
+      const int nb = t.n_blk * BN / 128 + (lane & 1);
+      const bool nb_ok = lane < Cfg::kSubs && nb * 128 < args.N;
+      const float* b_scale = args.b_scale + t.group * args.b_scale_group + nb * args.b_scale_n;
+      for (int kb = 0; kb < k_blocks; kb += Cfg::kScaleBlocks) {
+        const int s = n % Cfg::kScaleStages;
+        if (!wait_warp(scale_empty_bar(s), ((n / Cfg::kScaleStages) & 1u) ^ 1u, DEV_TIMEOUT_PRODUCER)) { ok = false; break; }
+#pragma unroll
+        for (int i = 0; i < Cfg::kScaleBlocks; ++i) {
+          const uint32_t dst = scale_base + s * Cfg::kScaleStageBytes + i * (BM + 4) * 4;
+          const bool in = kb + i < k_blocks;
+#pragma unroll
+          for (int r = lane; r < BM; r += 32)
+            ptx::copy_async_4(dst + r * 4, a_scale + (kb + i) * args.a_scale_ld + r, in && row0 + r < t.row_end);
+          if (lane < Cfg::kSubs) ptx::copy_async_4(dst + (BM + lane) * 4, b_scale + (kb + i) * args.b_scale_k, in && nb_ok);
+        }
+        ptx::copy_async_arrive(scale_full_bar(s));
+        ++n;
+      }
+    }
+  }
   } else {
-    // ------------------------------------------------------------------ epilogue (warps 2..9)
+    // ------------------------------------------------------------------ epilogue
+    if constexpr (Cfg::kScaled) ptx::registers_inc<Cfg::kEpilogueRegs>();
     const int q = warp & 3;
-    const int half = (warp - 2) >> 2;
-    const uint32_t stage_buf = store_base + (warp - 2) * Cfg::kStageOutBytes;
+    const int half = (warp - Cfg::kFirstEpilogueWarp) >> 2;
+    const uint32_t stage_buf = store_base + (warp - Cfg::kFirstEpilogueWarp) * Cfg::kStageOutBytes;
     constexpr int kChunks = (BN / 32 + 1) / 2;           // 32-column chunks of one epilogue warp: half, half + 2, ...
     GroupedIter<Cfg> it(worker, workers);
     GroupedTile t;
     uint32_t n_acc = 0;
+    [[maybe_unused]] uint32_t n_scale = 0;
     bool ok = true;
     while (ok && it.next(args, plan_first, plan_tiles, t)) {
       const int row0 = t.row0 + static_cast<int>(cta) * BM + q * 32;      // the warp's first row
@@ -488,59 +618,60 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       const int k_blocks = (t.k_len + BKE - 1) / BKE;
       const uint32_t lane_base = static_cast<uint32_t>(q * 32) << 16;
       [[maybe_unused]] float acc[Cfg::kScaled ? kChunks : 1][32];
-      uint32_t b = n_acc & 1u;
+      const uint32_t b = n_acc & 1u;
 
       if constexpr (Cfg::kScaled) {
 #pragma unroll
         for (int ci = 0; ci < kChunks; ++ci)
 #pragma unroll
           for (int i = 0; i < 32; ++i) acc[ci][i] = 0.0f;
-        const float* a_scale = args.a_scale + row;
-        const int nb0 = t.n_blk * BN / 128;
-        const int last_nb = (args.N - 1) / 128;
-        const float* b_scale = args.b_scale + t.group * args.b_scale_group + nb0 * args.b_scale_n;
-        const long long next_n = nb0 < last_nb ? args.b_scale_n : 0;       // second 128 columns of a 256-wide tile
-        float sa = 0.0f, sb0 = 0.0f, sb1 = 0.0f;
-        if (k_blocks > 0) {
-          sa = row_ok ? __ldg(a_scale) : 0.0f;
-          sb0 = __ldg(b_scale);
-          if (BN > 128) sb1 = __ldg(b_scale + next_n);
-        }
-        for (int kb = 0; kb < k_blocks; ++kb) {
-          const float s0 = sa * sb0, s1 = sa * sb1;
-          if (kb + 1 < k_blocks) {
-            // The next block's scales are on their way while this one is awaited.
-            sa = row_ok ? __ldg(a_scale + (kb + 1) * args.a_scale_ld) : 0.0f;
-            sb0 = __ldg(b_scale + (kb + 1) * args.b_scale_k);
-            if (BN > 128) sb1 = __ldg(b_scale + next_n + (kb + 1) * args.b_scale_k);
+        for (int kb = 0; kb < k_blocks && ok; ++kb) {
+          const int ss = n_scale % Cfg::kScaleStages;
+          const int in_stage = kb % Cfg::kScaleBlocks;
+          if (in_stage == 0 && !wait(scale_full_bar(ss), (n_scale / Cfg::kScaleStages) & 1u, DEV_TIMEOUT_EPILOGUE)) {
+            ok = false;
+            break;
           }
-          b = n_acc & 1u;
-          if (!wait(acc_full_bar(b), (n_acc >> 1) & 1u, DEV_TIMEOUT_EPILOGUE)) { ok = false; break; }
-          ptx::tc_fence_after_sync();
+          const float* scales = scale_ring + ss * (Cfg::kScaleStageBytes / 4) + in_stage * (BM + 4);
+          const float sa = scales[q * 32 + lane];
+          float sc[Cfg::kSubs];
 #pragma unroll
-          for (int ci = 0; ci < kChunks; ++ci) {
-            const int c = half + 2 * ci;
-            if (c < BN / 32) {
-              uint32_t r[32];
-              ptx::tmem_ld_32x32(tmem_base + lane_base + b * BN + c * 32, r);
-              ptx::tmem_ld_wait();
-              const float sc = (BN > 128 && c >= 4) ? s1 : s0;
+          for (int j = 0; j < Cfg::kSubs; ++j) sc[j] = sa * scales[BM + j];
+          if (in_stage + 1 == Cfg::kScaleBlocks || kb + 1 == k_blocks) {
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(scale_empty_bar(ss));
+            ++n_scale;
+          }
 #pragma unroll
-              for (int i = 0; i < 32; i += 2) {
-                const float2 f = actm::fma2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), actm::both(sc),
-                                            make_float2(acc[ci][i], acc[ci][i + 1]));
-                acc[ci][i] = f.x;
-                acc[ci][i + 1] = f.y;
+          for (int j = 0; j < Cfg::kSubs; ++j) {
+            const uint32_t d = n_acc % Cfg::kAccs;
+            if (!wait(acc_full_bar(d), (n_acc / Cfg::kAccs) & 1u, DEV_TIMEOUT_EPILOGUE)) { ok = false; break; }
+            ptx::tc_fence_after_sync();
+            constexpr int kPerSub = (Cfg::SUB / 32 + 1) / 2;
+#pragma unroll
+            for (int ci = j * kPerSub; ci < (j + 1) * kPerSub; ++ci) {
+              const int c = half + 2 * ci;
+              if (c < BN / 32) {
+                uint32_t r[32];
+                ptx::tmem_ld_32x32(tmem_base + lane_base + d * Cfg::SUB + c * 32 - j * Cfg::SUB, r);
+                ptx::tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                  const float2 f = actm::fma2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), actm::both(sc[j]),
+                                              make_float2(acc[ci][i], acc[ci][i + 1]));
+                  acc[ci][i] = f.x;
+                  acc[ci][i + 1] = f.y;
+                }
               }
             }
+            ptx::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (kPair) ptx::mbar_arrive_cluster_read(acc_empty_bar(d), 0);
+              else ptx::mbar_arrive(acc_empty_bar(d));
+            }
+            ++n_acc;
           }
-          ptx::tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) {
-            if constexpr (kPair) ptx::mbar_arrive_cluster(acc_empty_bar(b), 0);
-            else ptx::mbar_arrive(acc_empty_bar(b));
-          }
-          ++n_acc;
         }
         if (!ok) break;
       } else if (k_blocks > 0) {
@@ -554,13 +685,14 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         if (col0 >= args.N || row0 >= t.row_end) break;         // warp-uniform
         float v[32];
         if constexpr (Cfg::kScaled) {
-          // Registers cannot be indexed at run time: a chain of selections.
+          // The chunk is worked on in place of acc[0], then the others move up: with a copy beside all accumulators
+          // (and with 32 derivatives at a time, below) some of them were spilled in the loop over k-blocks too.
 #pragma unroll
-          for (int ci = 0; ci < kChunks; ++ci)
-            if (c == half + 2 * ci) {
+          for (int i = 0; i < 32; ++i) v[i] = acc[0][i];
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = acc[ci][i];
-            }
+          for (int ci = 0; ci + 1 < kChunks; ++ci)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) acc[ci][i] = acc[ci + 1][i];
         } else if (k_blocks > 0) {
           uint32_t r[32];
           ptx::tmem_ld_32x32(tmem_base + lane_base + b * BN + c * 32, r);
@@ -605,7 +737,13 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
             const char* bias = static_cast<const char*>(args.bias) + static_cast<long long>(t.group) * args.N * elt;
             add_bias_chunk(v, bias, args.bias_dtype, col0, valid, odt);
           }
-          if (args.aux != nullptr && args.save_grad) {
+          if (Cfg::kScaled && args.aux != nullptr && args.save_grad) {
+            if (row_ok) {
+              act_fwd_grad_slices(v, args.act, args.act_param, odt, [&](int i0, const float (&g)[8]) {
+                store_slice(args.aux, gdt, static_cast<long long>(row) * args.ld_aux + col0 + i0, g, valid - i0);
+              });
+            }
+          } else if (args.aux != nullptr && args.save_grad) {
             float zr[32], g[32];
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
@@ -628,7 +766,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         ptx::tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) {
-          if constexpr (kPair) ptx::mbar_arrive_cluster(acc_empty_bar(b), 0);
+          if constexpr (kPair) ptx::mbar_arrive_cluster_read(acc_empty_bar(b), 0);
           else ptx::mbar_arrive(acc_empty_bar(b));
         }
         ++n_acc;

@@ -60,7 +60,7 @@ int launch_grouped_cfg(const GroupedProblem& p, cudaStream_t stream) {
   else if (Cfg::B_MN)
     rc = encode_3d(&tb, elt, p.b, p.b_cols, p.b_rows, g.groups, p.b_pitch * elt, p.b_group_pitch * elt, Cfg::MN_ATOM, Cfg::BKE, sw_mn);
   else
-    rc = encode_3d(&tb, elt, p.b, p.b_cols, p.b_rows, g.groups, p.b_pitch * elt, p.b_group_pitch * elt, Cfg::BKE, Cfg::BN_CTA, sw);
+    rc = encode_3d(&tb, elt, p.b, p.b_cols, p.b_rows, g.groups, p.b_pitch * elt, p.b_group_pitch * elt, Cfg::BKE, Cfg::kSubs > 1 ? Cfg::SUB / Cfg::CTAS : Cfg::BN_CTA, sw);
   if (rc != OK) return rc;
 
   CUtensorMap tout = ta, taux = ta;
@@ -81,7 +81,7 @@ int launch_grouped_cfg(const GroupedProblem& p, cudaStream_t stream) {
   g.tiles_m = Cfg::kRaggedK ? (g.M + Cfg::TILE_M - 1) / Cfg::TILE_M : 0;
   g.group_m = raster_group_m() / Cfg::CTAS > 0 ? raster_group_m() / Cfg::CTAS : 1;
   const uint32_t fmt = Cfg::ELT == 1 ? 0u : (p.op_dtype == DT_F32 ? 2u : (p.op_dtype == DT_BF16 ? 1u : 0u));
-  g.idesc = ptx::make_idesc(fmt, Cfg::A_MN ? 1u : 0u, Cfg::B_MN ? 1u : 0u, Cfg::TILE_M, Cfg::BN);
+  g.idesc = ptx::make_idesc(fmt, Cfg::A_MN ? 1u : 0u, Cfg::B_MN ? 1u : 0u, Cfg::TILE_M, Cfg::SUB);
 
   // The most tiles this call can have: the split of the rows over the groups is known to the device only.
   const long long row_tiles = Cfg::kRaggedK ? static_cast<long long>(g.tiles_m) * g.groups

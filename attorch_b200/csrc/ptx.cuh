@@ -63,6 +63,29 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar, uint32_t cta) 
       : "memory");
 }
 
+// The same without cluster-wide release of this thread's earlier writes to memory (which waits for all of them: 1300
+// clocks where this was measured): for a barrier that says only that tensor memory has been read.
+__device__ __forceinline__ void mbar_arrive_cluster_read(uint32_t bar, uint32_t cta) {
+  asm volatile(
+      "{\n\t.reg .b32 remote;\n\t"
+      "mapa.shared::cluster.u32 remote, %0, %1;\n\t"
+      "mbarrier.arrive.shared::cluster.b64 _, [remote];\n\t}" ::"r"(bar),
+      "r"(cta)
+      : "memory");
+}
+
+// True in one lane of a converged warp.  Unlike a comparison of the lane number it leaves the branch's operands
+// in uniform registers, which is where tcgen05 instructions read them.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xFFFFFFFF;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(yes));
+  return yes != 0;
+}
+
 __device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
                : "memory");
@@ -91,6 +114,26 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t par
       : "r"(bar), "r"(parity)
       : "memory");
   return done != 0;
+}
+
+// Asynchronous copy of 4 bytes global -> shared, zeros if `in` is false (nothing is read then), and an arrival on an
+// mbarrier (counted in its expected arrivals) once this thread's copies so far have landed.
+__device__ __forceinline__ void copy_async_4(uint32_t smem_dst, const void* gmem_src, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_dst), "l"(gmem_src), "r"(in ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// Gives registers of this warpgroup back, or takes them from what other warpgroups of the block gave back (all four
+// warps of the warpgroup execute it; the shares add up to at most what the block was launched with).
+template <int kRegs>
+__device__ __forceinline__ void registers_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void registers_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
 // Longest time one mbarrier wait may take before a kernel gives up (nanoseconds of %globaltimer).
