@@ -115,10 +115,10 @@ struct GroupedCfg {
   static constexpr uint32_t MN_SBO = MN_BASE32 ? 512 : 1024;
   // 8-bit: 12 warps, the epilogue's two warpgroups (warps 4-11) take registers over from the first one: with
   // 168 a thread (384 threads at launch) part of the 128 accumulators lived in local memory, and a stage took 3 us
-  // instead of 0.3.  256 * 216 + 128 * 72 = 384 * 168.
+  // instead of 0.3.  256 * 224 + 128 * 56 = 384 * 168.
   static constexpr int kFirstEpilogueWarp = kScaled ? 4 : 2;
   static constexpr int kThreads = 32 * (kFirstEpilogueWarp + kEpilogueWarps);
-  static constexpr int kEpilogueRegs = 216, kOtherRegs = 72;
+  static constexpr int kEpilogueRegs = 224, kOtherRegs = 56;
   static constexpr int kBoxRows = 32;            // rows per box of a partly filled K-major A tile
   static_assert(BN % 32 == 0 && BN >= 32 && BN <= 256);
   static_assert(A_MN_ ? B_MN_ : true, "an MN-major A is the ragged reduction");
@@ -335,7 +335,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     }
     for (int b = 0; b < Cfg::kAccs; ++b) {
       ptx::mbar_init(acc_full_bar(b), 1);
-      ptx::mbar_init(acc_empty_bar(b), Cfg::kEpilogueWarps * CTAS);
+      ptx::mbar_init(acc_empty_bar(b), Cfg::kEpilogueWarps / Cfg::kSubs * CTAS);
     }
     if (Cfg::kScaled)
       for (int b = 0; b < Cfg::kScaleStages; ++b) {
@@ -365,7 +365,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   auto wait = [&](uint32_t bar, uint32_t parity, int code) -> bool {
     uint32_t spins = 0;
     uint64_t t0 = 0;
-    while (!(kPair ? ptx::mbar_try_wait_cluster(bar, parity) : ptx::mbar_try_wait(bar, parity))) {
+    // Only rows cleared by the other CTA of a pair (ragged reduction) are memory that a wait has to acquire from it.
+    while (!(kPair && Cfg::kRaggedK ? ptx::mbar_try_wait_cluster(bar, parity) : ptx::mbar_try_wait(bar, parity))) {
       if ((++spins & 0x3FFu) == 0) {
         if (*abort_flag) return false;
         const uint64_t now = ptx::globaltimer_ns();
@@ -459,10 +460,13 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         }
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 || (Cfg::kScaled && warp == 3)) {
     // ------------------------------------------------------------------ MMA issuer
     // The leader's warp walks the tiles converged and elects a lane to issue.  In the ragged reduction the other
-    // CTA's does too, to clear the rows behind a group's end in its own shared memory.
+    // CTA's does too, to clear the rows behind a group's end in its own shared memory.  With scales every k-block is
+    // an accumulation of its own, so two warps issue alternate ones: waiting and issuing take one warp 700 clocks a
+    // k-block, more than a narrow tile's MMA and loads do.
+    const int own = Cfg::kScaled && warp == 3 ? 1 : 0;
     auto issuer_wait = [&](uint32_t bar, uint32_t parity) -> bool {
       return __all_sync(0xFFFFFFFFu, wait(bar, parity, DEV_TIMEOUT_MMA));
     };
@@ -472,6 +476,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       int s = 0;
       uint32_t ph = 0;
       uint32_t tail_ph = 0;                   // bit s: parity of tail_bar(s)
+      [[maybe_unused]] int n_block = 0;
       uint32_t n_acc = 0;
       bool ok = true;
       while (ok && it.next(args, plan_first, plan_tiles, t)) {
@@ -483,6 +488,11 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
           ptx::tc_fence_after_sync();
         }
         for (int kb = 0; kb < k_blocks; ++kb) {
+          if (Cfg::kScaled && (n_block++ & 1) != own) {
+            n_acc += Cfg::kSubs;
+            if (++s == STAGES) { s = 0; ph ^= 1u; }
+            continue;
+          }
           const uint32_t a_addr = smem_base + s * Cfg::STAGE_BYTES;
           const uint32_t b_addr = a_addr + Cfg::A_BYTES;
           if constexpr (Cfg::kRaggedK) {
@@ -604,7 +614,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     const int q = warp & 3;
     const int half = (warp - Cfg::kFirstEpilogueWarp) >> 2;
     const uint32_t stage_buf = store_base + (warp - Cfg::kFirstEpilogueWarp) * Cfg::kStageOutBytes;
-    constexpr int kChunks = (BN / 32 + 1) / 2;           // 32-column chunks of one epilogue warp: half, half + 2, ...
+    // 32-column chunks of one epilogue warp: every other one, or, of a tile in two parts, those of one part.
+    constexpr int kChunks = (BN / 32 + 1) / 2;
+    auto chunk_at = [&](int i) { return Cfg::kSubs > 1 ? half * kChunks + i : half + 2 * i; };
     GroupedIter<Cfg> it(worker, workers);
     GroupedTile t;
     uint32_t n_acc = 0;
@@ -634,43 +646,49 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
           }
           const float* scales = scale_ring + ss * (Cfg::kScaleStageBytes / 4) + in_stage * (BM + 4);
           const float sa = scales[q * 32 + lane];
-          float sc[Cfg::kSubs];
-#pragma unroll
-          for (int j = 0; j < Cfg::kSubs; ++j) sc[j] = sa * scales[BM + j];
+          const float sc = sa * scales[BM + (Cfg::kSubs > 1 ? half : 0)];
           if (in_stage + 1 == Cfg::kScaleBlocks || kb + 1 == k_blocks) {
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(scale_empty_bar(ss));
             ++n_scale;
           }
+          // This k-block's part for this warp: with two parts the quarter's warps take one each, else they share it.
+          const uint32_t d = (n_acc + (Cfg::kSubs > 1 ? half : 0)) % Cfg::kAccs;
+          if (!wait(acc_full_bar(d), (n_acc / Cfg::kAccs) & 1u, DEV_TIMEOUT_EPILOGUE)) { ok = false; break; }
+          n_acc += Cfg::kSubs;
+          ptx::tc_fence_after_sync();
+          // The accumulator is handed back before the last arithmetic.  A warp without rows only hands it back.  Two chunks
+          // are loaded together where they are all; of four, more than one at a time cost registers (spills: 197
+          // against 184 us at 8192 x 4096 x 4096).
+          constexpr int kTwo = kChunks == 2 ? 2 : 1;
 #pragma unroll
-          for (int j = 0; j < Cfg::kSubs; ++j) {
-            const uint32_t d = n_acc % Cfg::kAccs;
-            if (!wait(acc_full_bar(d), (n_acc / Cfg::kAccs) & 1u, DEV_TIMEOUT_EPILOGUE)) { ok = false; break; }
-            ptx::tc_fence_after_sync();
-            constexpr int kPerSub = (Cfg::SUB / 32 + 1) / 2;
+          for (int c0 = 0; c0 < kChunks; c0 += kTwo) {
+            uint32_t r[kTwo][32];
 #pragma unroll
-            for (int ci = j * kPerSub; ci < (j + 1) * kPerSub; ++ci) {
-              const int c = half + 2 * ci;
-              if (c < BN / 32) {
-                uint32_t r[32];
-                ptx::tmem_ld_32x32(tmem_base + lane_base + d * Cfg::SUB + c * 32 - j * Cfg::SUB, r);
-                ptx::tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                  const float2 f = actm::fma2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), actm::both(sc[j]),
-                                              make_float2(acc[ci][i], acc[ci][i + 1]));
-                  acc[ci][i] = f.x;
-                  acc[ci][i + 1] = f.y;
-                }
+            for (int i = 0; i < kTwo; ++i)
+              if (chunk_at(c0 + i) < BN / 32 && row0 < t.row_end)
+                ptx::tmem_ld_32x32(tmem_base + lane_base + d * Cfg::SUB + (chunk_at(c0 + i) % (Cfg::SUB / 32)) * 32, r[i]);
+            ptx::tmem_ld_wait();
+            if (c0 + kTwo >= kChunks) {
+              ptx::tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) {
+                if constexpr (kPair) ptx::mbar_arrive_cluster_read(acc_empty_bar(d), 0);
+                else ptx::mbar_arrive(acc_empty_bar(d));
               }
             }
-            ptx::tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-              if constexpr (kPair) ptx::mbar_arrive_cluster_read(acc_empty_bar(d), 0);
-              else ptx::mbar_arrive(acc_empty_bar(d));
-            }
-            ++n_acc;
+#pragma unroll
+            for (int i = 0; i < kTwo; ++i)
+              if (chunk_at(c0 + i) < BN / 32 && row0 < t.row_end) {
+                float (&sum)[32] = acc[c0 + i];
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                  const float2 f = actm::fma2(make_float2(__uint_as_float(r[i][e]), __uint_as_float(r[i][e + 1])),
+                                              actm::both(sc), make_float2(sum[e], sum[e + 1]));
+                  sum[e] = f.x;
+                  sum[e + 1] = f.y;
+                }
+              }
           }
         }
         if (!ok) break;
@@ -680,9 +698,10 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       }
 
 #pragma unroll 1
-      for (int c = half; c < BN / 32; c += 2) {
+      for (int ci = 0; ci < kChunks; ++ci) {
+        const int c = chunk_at(ci);
         const int col0 = t.n_blk * BN + c * 32;
-        if (col0 >= args.N || row0 >= t.row_end) break;         // warp-uniform
+        if (c >= BN / 32 || col0 >= args.N || row0 >= t.row_end) break;         // warp-uniform
         float v[32];
         if constexpr (Cfg::kScaled) {
           // The chunk is worked on in place of acc[0], then the others move up: with a copy beside all accumulators
@@ -690,9 +709,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = acc[0][i];
 #pragma unroll
-          for (int ci = 0; ci + 1 < kChunks; ++ci)
+          for (int k = 0; k + 1 < kChunks; ++k)
 #pragma unroll
-            for (int i = 0; i < 32; ++i) acc[ci][i] = acc[ci + 1][i];
+            for (int i = 0; i < 32; ++i) acc[k][i] = acc[k + 1][i];
         } else if (k_blocks > 0) {
           uint32_t r[32];
           ptx::tmem_ld_32x32(tmem_base + lane_base + b * BN + c * 32, r);
