@@ -396,7 +396,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   if constexpr (Cfg::kScaled) ptx::registers_dec<Cfg::kOtherRegs>();
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
-    if (lane == 0) {
+    // The warp walks converged and elects a lane (see the issuer): one lane in a branch of its own took 600 clocks a stage.
+    {
       GroupedIter<Cfg> it(worker, workers);
       GroupedTile t;
       int s = 0;
@@ -412,50 +413,53 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
           a_bytes = a_tile_bytes<Cfg>(t.row_end - m0);
           pair_a_bytes = a_tile_bytes<Cfg>(t.row_end - t.row0) + (kPair ? a_tile_bytes<Cfg>(t.row_end - t.row0 - BM) : 0u);
         }
+        const uint32_t expect = (kPair ? pair_a_bytes : a_bytes) + Cfg::B_BYTES * CTAS;
         for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!wait(empty_bar(s), ph ^ 1u, DEV_TIMEOUT_PRODUCER)) { ok = false; break; }
-          const int k0 = kb * BKE;
-          const bool tail = Cfg::kRaggedK && k0 + BKE > t.k_len;
-          uint32_t full = full_bar(s);
-          if (tail) {
-            full = tail_bar(s);
-            ptx::mbar_arrive_expect_tx(full, Cfg::STAGE_BYTES);
-            if constexpr (kPair) full = ptx::map_to_cta(full, cta);
-          } else if constexpr (kPair) {
-            if (cta == 0) ptx::mbar_arrive_expect_tx(full, pair_a_bytes + Cfg::B_BYTES * CTAS);
-            full = ptx::map_to_cta(full, 0);
-          } else {
-            ptx::mbar_arrive_expect_tx(full, a_bytes + Cfg::B_BYTES);
+          if (!__all_sync(0xFFFFFFFFu, wait(empty_bar(s), ph ^ 1u, DEV_TIMEOUT_PRODUCER))) { ok = false; break; }
+          if (ptx::elect_one()) {
+            const int k0 = kb * BKE;
+            uint32_t full = full_bar(s);
+            if (Cfg::kRaggedK && k0 + BKE > t.k_len) {
+              full = tail_bar(s);
+              ptx::mbar_arrive_expect_tx(full, Cfg::STAGE_BYTES);
+              if constexpr (kPair) full = ptx::map_to_cta(full, cta);
+            } else {
+              if (cta == 0) ptx::mbar_arrive_expect_tx(full, expect);
+              if constexpr (kPair) full = ptx::map_to_cta(full, 0);
+            }
+            const uint32_t a_dst = smem_base + s * Cfg::STAGE_BYTES;
+            const uint32_t b_dst = a_dst + Cfg::A_BYTES;
+            if constexpr (Cfg::A_MN) {
+#pragma unroll
+              for (int j = 0; j < BM / Cfg::MN_ATOM; ++j)
+                ptx::tma_load_2d<kPair>(a_dst + j * Cfg::MN_BOX_BYTES, &tmap_a, full, m0 + j * Cfg::MN_ATOM, t.k_row0 + k0);
+            } else if (a_bytes == Cfg::A_BYTES) {
+              ptx::tma_load_2d<kPair>(a_dst, &tmap_a, full, k0, m0);
+            } else {
+#pragma unroll
+              for (int j = 0; j < BM / Cfg::kBoxRows; ++j)
+                if (j * Cfg::kBoxRows * 128u < a_bytes)
+                  ptx::tma_load_2d<kPair>(a_dst + j * Cfg::kBoxRows * 128, &tmap_a_box, full, k0, m0 + j * Cfg::kBoxRows);
+            }
+            if constexpr (Cfg::kRaggedK) {
+#pragma unroll
+              for (int j = 0; j < Cfg::BN_CTA / Cfg::MN_ATOM; ++j)
+                ptx::tma_load_2d<kPair>(b_dst + j * Cfg::MN_BOX_BYTES, &tmap_b, full, n0 + j * Cfg::MN_ATOM, t.k_row0 + k0);
+            } else if constexpr (Cfg::B_MN) {
+#pragma unroll
+              for (int j = 0; j < Cfg::BN_CTA / Cfg::MN_ATOM; ++j)
+                ptx::tma_load_3d<kPair>(b_dst + j * Cfg::MN_BOX_BYTES, &tmap_b, full, n0 + j * Cfg::MN_ATOM, k0, t.group);
+            } else if constexpr (kPair && Cfg::kSubs > 1) {
+              // Each 128-column part of the tile is a product of its own, of which each CTA holds half the columns.
+#pragma unroll
+              for (int j = 0; j < Cfg::kSubs; ++j)
+                ptx::tma_load_3d<kPair>(b_dst + j * (Cfg::SUB / CTAS) * 128, &tmap_b, full, k0,
+                                        t.n_blk * BN + j * Cfg::SUB + static_cast<int>(cta) * (Cfg::SUB / CTAS), t.group);
+            } else {
+              ptx::tma_load_3d<kPair>(b_dst, &tmap_b, full, k0, n0, t.group);
+            }
           }
-          const uint32_t a_dst = smem_base + s * Cfg::STAGE_BYTES;
-          const uint32_t b_dst = a_dst + Cfg::A_BYTES;
-          if constexpr (Cfg::A_MN) {
-#pragma unroll
-            for (int j = 0; j < BM / Cfg::MN_ATOM; ++j)
-              ptx::tma_load_2d<kPair>(a_dst + j * Cfg::MN_BOX_BYTES, &tmap_a, full, m0 + j * Cfg::MN_ATOM, t.k_row0 + k0);
-          } else if (a_bytes == Cfg::A_BYTES) {
-            ptx::tma_load_2d<kPair>(a_dst, &tmap_a, full, k0, m0);
-          } else {
-            for (uint32_t off = 0; off < a_bytes; off += Cfg::kBoxRows * 128)
-              ptx::tma_load_2d<kPair>(a_dst + off, &tmap_a_box, full, k0, m0 + static_cast<int>(off / 128));
-          }
-          if constexpr (Cfg::kRaggedK) {
-#pragma unroll
-            for (int j = 0; j < Cfg::BN_CTA / Cfg::MN_ATOM; ++j)
-              ptx::tma_load_2d<kPair>(b_dst + j * Cfg::MN_BOX_BYTES, &tmap_b, full, n0 + j * Cfg::MN_ATOM, t.k_row0 + k0);
-          } else if constexpr (Cfg::B_MN) {
-#pragma unroll
-            for (int j = 0; j < Cfg::BN_CTA / Cfg::MN_ATOM; ++j)
-              ptx::tma_load_3d<kPair>(b_dst + j * Cfg::MN_BOX_BYTES, &tmap_b, full, n0 + j * Cfg::MN_ATOM, k0, t.group);
-          } else if constexpr (Cfg::kSubs > 1) {
-            // Each 128-column part of the tile is a product of its own: of a pair, each CTA holds half of its columns.
-#pragma unroll
-            for (int j = 0; j < Cfg::kSubs; ++j)
-              ptx::tma_load_3d<kPair>(b_dst + j * (Cfg::SUB / CTAS) * 128, &tmap_b, full, k0,
-                                      t.n_blk * BN + j * Cfg::SUB + static_cast<int>(cta) * (Cfg::SUB / CTAS), t.group);
-          } else {
-            ptx::tma_load_3d<kPair>(b_dst, &tmap_b, full, k0, n0, t.group);
-          }
+          __syncwarp();
           if (++s == STAGES) { s = 0; ph ^= 1u; }
         }
       }

@@ -60,7 +60,7 @@ int launch_grouped_cfg(const GroupedProblem& p, cudaStream_t stream) {
   else if (Cfg::B_MN)
     rc = encode_3d(&tb, elt, p.b, p.b_cols, p.b_rows, g.groups, p.b_pitch * elt, p.b_group_pitch * elt, Cfg::MN_ATOM, Cfg::BKE, sw_mn);
   else
-    rc = encode_3d(&tb, elt, p.b, p.b_cols, p.b_rows, g.groups, p.b_pitch * elt, p.b_group_pitch * elt, Cfg::BKE, Cfg::kSubs > 1 ? Cfg::SUB / Cfg::CTAS : Cfg::BN_CTA, sw);
+    rc = encode_3d(&tb, elt, p.b, p.b_cols, p.b_rows, g.groups, p.b_pitch * elt, p.b_group_pitch * elt, Cfg::BKE, Cfg::CTAS > 1 && Cfg::kSubs > 1 ? Cfg::SUB / Cfg::CTAS : Cfg::BN_CTA, sw);
   if (rc != OK) return rc;
 
   CUtensorMap tout = ta, taux = ta;

@@ -14,7 +14,8 @@ import torch
 from torch import Tensor, nn
 
 from . import _lib
-from .linear_layer import (Linear, _as_operand, _cached_size, _dtype_id, _flags_for, _ptr, _require_cuda, _stream_scratch,
+from ._launch import on, status_of, stream_of
+from .linear_layer import (Linear, _as_operand, _cached_size, _dtype_id, _flags_for, _ptr, _require_cuda,
                            get_output_dtype)
 
 MAX_EXPERTS, MAX_TOP_K = 512, 32
@@ -70,8 +71,8 @@ def _route(logits: Tensor, top_k: int, score_func: str, renormalize: bool, mask:
     dtype = _dtype_id(logits.dtype)
     logits = _inner_unit(logits)
     lib = _lib.load()
-    with torch.cuda.device(device):
-        stream = torch.cuda.current_stream().cuda_stream
+    with on(device):
+        stream = stream_of(device)
         weights = torch.empty((tokens, top_k), dtype=torch.float32, device=device)
         # Whole numbers share one allocation; the C entry takes their addresses.
         slots = tokens * top_k
@@ -107,8 +108,8 @@ class RouteAutoGrad(torch.autograd.Function):
         logits, weights, chosen, stats = ctx.saved_tensors
         tokens, experts = logits.shape
         lib = _lib.load()
-        with torch.cuda.device(logits.device):
-            stream = torch.cuda.current_stream().cuda_stream
+        with on(logits.device):
+            stream = stream_of(logits.device)
             grad = weights_grad.float().contiguous()
             logits_grad = torch.empty((tokens, experts), dtype=logits.dtype, device=logits.device)
             _lib.check(lib.ab200_route_backward(
@@ -154,8 +155,8 @@ def _dispatch(input: Tensor, token_row: Tensor, offsets: Tensor) -> Tensor:
     tokens, top_k = token_row.shape
     x = _inner_unit(input)
     lib = _lib.load()
-    with torch.cuda.device(x.device):
-        stream = torch.cuda.current_stream().cuda_stream
+    with on(x.device):
+        stream = stream_of(x.device)
         rows = torch.empty((tokens * top_k, x.shape[1]), dtype=x.dtype, device=x.device)
         _lib.check(lib.ab200_expert_dispatch(_ptr(x), _ptr(token_row), _row_end(offsets), _ptr(rows), tokens, top_k,
                                              tokens * top_k, x.shape[1], _pitch(x), _dtype_id(x.dtype), stream),
@@ -167,8 +168,8 @@ def _combine(rows: Tensor, token_row: Tensor, weights: Optional[Tensor]) -> Tens
     tokens, top_k = token_row.shape
     rows = _inner_unit(rows)
     lib = _lib.load()
-    with torch.cuda.device(rows.device):
-        stream = torch.cuda.current_stream().cuda_stream
+    with on(rows.device):
+        stream = stream_of(rows.device)
         output = torch.empty((tokens, rows.shape[1]), dtype=rows.dtype, device=rows.device)
         _lib.check(lib.ab200_expert_combine(_ptr(rows), _ptr(token_row), _ptr(weights), _ptr(output), tokens, top_k,
                                             rows.shape[0], rows.shape[1], _pitch(rows), _dtype_id(rows.dtype), stream),
@@ -202,8 +203,8 @@ class CombineAutoGrad(torch.autograd.Function):
         rows, weights, token_row, offsets = ctx.saved_tensors
         tokens, top_k = token_row.shape
         lib = _lib.load()
-        with torch.cuda.device(rows.device):
-            stream = torch.cuda.current_stream().cuda_stream
+        with on(rows.device):
+            stream = stream_of(rows.device)
             grad = _inner_unit(output_grad)
             rows = _inner_unit(rows)
             num_rows, dim = rows.shape
@@ -268,14 +269,14 @@ class GateAutoGrad(torch.autograd.Function):
         experts = weight.shape[1]
         dtype = get_output_dtype(input.dtype)
         lib = _lib.load()
-        with torch.cuda.device(input.device):
-            stream = torch.cuda.current_stream().cuda_stream
+        with on(input.device):
+            stream = stream_of(input.device)
             x_op = _inner_unit(_as_operand(input, dtype, stream))
             w_op = _inner_unit(_as_operand(weight, dtype, stream))
             output = torch.empty((rows, experts), dtype=dtype, device=input.device)
             _lib.check(lib.ab200_grouped_linear_forward(
                 _ptr(x_op), _ptr(w_op), None, None, None, _ptr(output), rows, 1, in_dim, experts, _pitch(x_op), 0, _pitch(w_op),
-                experts, experts, _dtype_id(dtype), 0, _lib.ACT_NONE, 0.0, _ptr(_stream_scratch(input.device)['status']), stream,
+                experts, experts, _dtype_id(dtype), 0, _lib.ACT_NONE, 0.0, status_of(input.device, stream), stream,
                 _flags_for(input.device)), 'ab200_grouped_linear_forward')
         ctx.dtypes = (input.dtype, weight.dtype)
         ctx.needs = (input.requires_grad, weight.requires_grad)
@@ -289,9 +290,9 @@ class GateAutoGrad(torch.autograd.Function):
         experts, dtype, device = w_op.shape[1], x_op.dtype, x_op.device
         lib = _lib.load()
         input_grad = weight_grad = None
-        with torch.cuda.device(device):
-            stream = torch.cuda.current_stream().cuda_stream
-            status = _ptr(_stream_scratch(device)['status'])
+        with on(device):
+            stream = stream_of(device)
+            status = status_of(device, stream)
             dy = _inner_unit(_as_operand(output_grad, dtype, stream))
             dt = _dtype_id(dtype)
 

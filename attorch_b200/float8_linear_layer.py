@@ -19,9 +19,10 @@ import torch
 from torch import Tensor, nn
 
 from . import _lib
+from ._launch import on, status_of, stream_of
 from .acts import act_id, parse_act_func
 from .grouped_linear_layer import MAX_GROUPS, GroupedLinear, _check_offsets, _pitch
-from .linear_layer import (Linear, _as_operand, _cached_size, _dtype_id, _flags_for, _ptr, _require_cuda, _stream_scratch,
+from .linear_layer import (Linear, _as_operand, _cached_size, _dtype_id, _flags_for, _ptr, _require_cuda,
                            _workspace, get_output_dtype)
 
 BLOCK = 128
@@ -80,8 +81,8 @@ def quantize_weight(weight: Tensor) -> Tuple[Tensor, Tensor]:
     """
     assert weight.ndim in (2, 3), f'Weights must be 2D or 3D, received shape {weight.shape}'
     _require_cuda(weight, 'weight')
-    with torch.no_grad(), torch.cuda.device(weight.device):
-        _, q_t, scale = _quantize_weight(weight.detach(), False, True, torch.cuda.current_stream().cuda_stream)
+    with torch.no_grad(), on(weight.device):
+        _, q_t, scale = _quantize_weight(weight.detach(), False, True, stream_of(weight.device))
     return q_t, scale
 
 
@@ -111,7 +112,7 @@ def _product(xq: Tensor, x_scale: Tensor, wq: Tensor, w_scale: Tensor, scale_str
         _ptr(xq), _ptr(x_scale), _ptr(wq), _ptr(w_scale), _ptr(bias), _ptr(offsets), _ptr(pre_act), _ptr(out), rows,
         wq.shape[0] if grouped else 1, k, n, _padded(k), x_scale.shape[1], wq.stride(0) if grouped and wq.shape[0] > 1 else n * pitch,
         pitch, *scale_strides, n, n, _dtype_id(out.dtype), _dtype_id(bias.dtype) if bias is not None else 0, act, param,
-        _ptr(_stream_scratch(device)['status']), stream, _flags_for(device) | extra_flags), 'ab200_float8_product')
+        status_of(device, stream), stream, _flags_for(device) | extra_flags), 'ab200_float8_product')
 
 
 def _check_stored(input: Tensor, weight: Tensor, scale: Tensor, bias: Optional[Tensor], ndim: int) -> None:
@@ -139,8 +140,8 @@ def _stored(input: Tensor, offsets: Optional[Tensor], weight: Tensor, scale: Ten
     flat = input.flatten(0, -2)
     out_dtype = get_output_dtype(input.dtype)
     _dtype_id(input.dtype)
-    with torch.cuda.device(input.device):
-        stream = torch.cuda.current_stream().cuda_stream
+    with on(input.device):
+        stream = stream_of(input.device)
         output = torch.empty((flat.shape[0], n), dtype=out_dtype, device=input.device)
         if output.numel():
             xq, x_scale = _quantize_rows(flat, stream)
@@ -207,8 +208,8 @@ class Float8LinearAutoGrad(torch.autograd.Function):
         rows, in_dim = flat.shape
         out_dim = weight.shape[1]
         out_dtype = get_output_dtype(input.dtype)
-        with torch.cuda.device(input.device):
-            stream = torch.cuda.current_stream().cuda_stream
+        with on(input.device):
+            stream = stream_of(input.device)
             x_op = _as_operand(flat, out_dtype, stream)
             if x_op.shape[1] > 1 and x_op.stride(1) != 1 or (rows > 1 and x_op.stride(0) < in_dim):
                 x_op = x_op.contiguous()
@@ -238,9 +239,9 @@ class Float8LinearAutoGrad(torch.autograd.Function):
         device, dtype = output_grad.device, output_grad.dtype
         lib = _lib.load()
         input_grad = weight_grad = bias_grad = None
-        with torch.cuda.device(device):
-            stream = torch.cuda.current_stream().cuda_stream
-            status = _ptr(_stream_scratch(device)['status'])
+        with on(device):
+            stream = stream_of(device)
+            status = status_of(device, stream)
             dt = _dtype_id(dtype)
             dy = _as_operand(output_grad.reshape(rows, out_dim), dtype, stream)
             if (out_dim > 1 and dy.stride(1) != 1) or (rows > 1 and dy.stride(0) < out_dim):

@@ -17,8 +17,9 @@ import torch
 from torch import Tensor, nn
 
 from . import _lib
+from ._launch import on, status_of, stream_of
 from .acts import act_id, parse_act_func
-from .linear_layer import _cached_size, _dtype_id, _flags_for, _ptr, _require_cuda, _stream_scratch, get_output_dtype
+from .linear_layer import _cached_size, _dtype_id, _flags_for, _ptr, _require_cuda, get_output_dtype
 
 MAX_GROUPS = 512
 
@@ -93,9 +94,9 @@ def _forward(input: Tensor, offsets: Tensor, weight: Tensor, bias: Optional[Tens
     rows = input.shape[0]
     out_dtype = get_output_dtype(input.dtype)
     lib = _lib.load()
-    with torch.cuda.device(input.device):
-        stream = torch.cuda.current_stream().cuda_stream
-        status = _ptr(_stream_scratch(input.device)['status'])
+    with on(input.device):
+        stream = stream_of(input.device)
+        status = status_of(input.device, stream)
         x_op = _rows_operand(input, out_dtype, stream)
         w_op = _stack_operand(weight, out_dtype, stream)
         bias_op = bias if bias is None or bias.is_contiguous() else bias.contiguous()
@@ -135,9 +136,9 @@ class GroupedLinearAutoGrad(torch.autograd.Function):
         dt = _dtype_id(dtype)
         lib = _lib.load()
         input_grad = weight_grad = bias_grad = None
-        with torch.cuda.device(device):
-            stream = torch.cuda.current_stream().cuda_stream
-            status = _ptr(_stream_scratch(device)['status'])
+        with on(device):
+            stream = stream_of(device)
+            status = status_of(device, stream)
             flags = _flags_for(device)
             dy = _rows_operand(output_grad, dtype, stream)
             dz = dy
