@@ -62,19 +62,44 @@ struct Tile {
   int bn;
   bool pair;
 };
+// A tile shape and the time of one k-block of a round of them (all SMs busy), in microseconds, measured on B200:
+// rounds of the same products forced to each shape (K = 4096 ... 8192, up to a few row tiles a group).
+struct TileCost {
+  int bn;
+  bool pair;
+  double cost;
+};
+constexpr TileCost kCosts16[] = {{256, true, 0.42}, {256, false, 0.50}, {128, false, 0.42}, {64, false, 0.38}};
+constexpr TileCost kCosts8[] = {{256, true, 0.65}, {128, false, 0.38}, {64, false, 0.33}, {32, false, 0.31}};
 
-// Tile of a product with ragged rows.  Every group with rows has at least one row tile, so the expected
-// number of row tiles of `tile_m` rows is about rows / tile_m + half a tile per group that can have rows.
-// Pairs (256 x 256) want whole tiles: an average of 256 rows a group.  Below that, the widest
-// tile that still gives every SM one.
-Tile pick_tile(int64_t rows, int64_t groups, int64_t N, bool allow_pair, int narrowest) {
+// The shape with the least rounds x cost; equal ones by the order above.  row_tiles(tile_m): expected row tiles of
+// that many rows.  Example: 3001 rows in 7 groups, 1000 columns: pairs 25 -> 19 us against 128-wide tiles; 4096 rows in
+// 32 groups, 2048 columns: 8-bit 128-wide 74 us, 64-wide 118 us, 32-wide 219 us.
+template <int kCount, class F>
+Tile pick_tile(const TileCost (&costs)[kCount], int64_t N, bool allow_pair, F&& row_tiles) {
+  Tile best{costs[kCount - 1].bn, false};
+  double least = -1.0;
+  for (const TileCost& c : costs) {
+    if (c.pair && !allow_pair) continue;
+    const int64_t tiles = row_tiles(c.pair ? 256 : 128) * ((N + c.bn - 1) / c.bn);
+    const int64_t workers = c.pair ? sm_count() / 2 : sm_count();
+    const double time = static_cast<double>((tiles + workers - 1) / workers) * c.cost;
+    if (least < 0.0 || time < least) {
+      least = time;
+      best = {c.bn, c.pair};
+    }
+  }
+  return best;
+}
+
+// Ragged rows: the host knows their number but not how they fall into groups.  Every group that can have rows has at
+// least one tile, and about half a tile more than its rows fill.
+auto ragged_row_tiles(int64_t rows, int64_t groups) {
   const int64_t used = groups < rows ? groups : rows;
-  if (allow_pair && N > 128 && rows >= 256 * groups && (rows / 256 + used / 2) * ((N + 255) / 256) * 2 >= sm_count())
-    return {256, true};
-  const int64_t row_tiles = rows / 128 + (used + 1) / 2 > used ? rows / 128 + (used + 1) / 2 : used;
-  int bn = 256;
-  while (bn > narrowest && (row_tiles * ((N + bn - 1) / bn) < sm_count() || N <= bn / 2)) bn /= 2;
-  return {bn, false};
+  return [=](int tile_m) {
+    const int64_t tiles = rows / tile_m + (used + 1) / 2;
+    return tiles > used ? tiles : used;
+  };
 }
 
 GroupedProblem grouped_problem(int op_dtype, int flags, int* status) {
@@ -148,7 +173,7 @@ int ab200_grouped_linear_forward(const void* x, const void* w, const void* bias,
   }
   p.a = x; p.a_pitch = ld_x;
   p.b = w; p.b_pitch = ld_w; p.b_group_pitch = w_group_stride; p.b_rows = g.K; p.b_cols = g.N;
-  const Tile t = pick_tile(rows, groups, N, p.allow_pair, 64);
+  const Tile t = pick_tile(kCosts16, N, p.allow_pair, ragged_row_tiles(rows, groups));
   set_last_path(AB200_PATH_TCGEN05);
   return dtype == DT_F32 ? launch_grouped_forward_32(p, t.bn, t.pair, stream) : launch_grouped_forward_16(p, t.bn, t.pair, stream);
 }
@@ -182,7 +207,7 @@ int ab200_grouped_linear_backward_input(const void* dz, const void* w, const int
   }
   p.a = dz; p.a_pitch = ld_dz;
   p.b = w; p.b_pitch = ld_w; p.b_group_pitch = w_group_stride; p.b_rows = static_cast<int>(K); p.b_cols = static_cast<int>(N);
-  const Tile t = pick_tile(rows, groups, K, p.allow_pair, 64);
+  const Tile t = pick_tile(kCosts16, K, p.allow_pair, ragged_row_tiles(rows, groups));
   set_last_path(AB200_PATH_TCGEN05);
   return dtype == DT_F32 ? launch_grouped_input_32(p, t.bn, t.pair, stream) : launch_grouped_input_16(p, t.bn, t.pair, stream);
 }
@@ -219,11 +244,8 @@ int ab200_grouped_linear_backward_weight(const void* x, const void* dz, const in
   }
   p.a = x; p.a_pitch = ld_x;
   p.b = dz; p.b_pitch = ld_dz;
-  // Every weight has the same tiles; pairs where they give every pair one.
-  const int64_t pairs = groups * ((K + 255) / 256) * ((N + 255) / 256);
-  Tile t{256, p.allow_pair && N > 128 && K > 128 && pairs * 2 >= sm_count()};
-  if (!t.pair)
-    while (t.bn > 64 && (groups * ((K + 127) / 128) * ((N + t.bn - 1) / t.bn) < sm_count() || N <= t.bn / 2)) t.bn /= 2;
+  // Every weight has the same tiles.
+  const Tile t = pick_tile(kCosts16, N, p.allow_pair, [=](int tile_m) { return groups * ((K + tile_m - 1) / tile_m); });
   set_last_path(AB200_PATH_TCGEN05);
   return dtype == DT_F32 ? launch_grouped_weight_32(p, t.bn, t.pair, stream) : launch_grouped_weight_16(p, t.bn, t.pair, stream);
 }
@@ -424,13 +446,21 @@ int ab200_expert_combine(const void* rows_in, const int* token_row, const float*
   const int64_t units = dim / per;
   const dim3 block = row_block(units);
   const unsigned grid = row_grid(tokens, block, 16);
-#define AB200_COMBINE(T, V)                                                                                                   \
-  combine_kernel<T, V><<<grid, block, 0, stream>>>(static_cast<const T*>(rows_in), ld_rows, token_row, weights,               \
+  if (rows == 0) return cudaMemsetAsync(y, 0, static_cast<size_t>(tokens) * dim * elt, stream) == cudaSuccess ? OK : ERR_LAUNCH;
+#define AB200_COMBINE_K(T, V, K)                                                                                              \
+  combine_kernel<T, V, K><<<grid, block, 0, stream>>>(static_cast<const T*>(rows_in), ld_rows, token_row, weights,            \
       static_cast<T*>(y), dim, static_cast<int>(tokens), static_cast<int>(top_k), static_cast<int>(rows), static_cast<int>(units))
+#define AB200_COMBINE(T, V)                          \
+  do {                                               \
+    if (top_k <= 2) AB200_COMBINE_K(T, V, 2);        \
+    else if (top_k <= 4) AB200_COMBINE_K(T, V, 4);   \
+    else AB200_COMBINE_K(T, V, 8);                   \
+  } while (0)
   if (dtype == DT_F32) { if (vec) AB200_COMBINE(float, 4); else AB200_COMBINE(float, 1); }
   else if (dtype == DT_F16) { if (vec) AB200_COMBINE(__half, 8); else AB200_COMBINE(__half, 1); }
   else { if (vec) AB200_COMBINE(__nv_bfloat16, 8); else AB200_COMBINE(__nv_bfloat16, 1); }
 #undef AB200_COMBINE
+#undef AB200_COMBINE_K
   return launched();
 }
 
@@ -475,7 +505,7 @@ int ab200_float8_quantize_rows(const void* x, void* q, float* scale, int64_t row
   if (ld_x < cols || ld_q < cols || ld_scale < rows || !aligned16(q, ld_q, 1)) return ERR_BAD_STRIDE;
   const bool vec = aligned16(x, ld_x, dtype_size(dtype));
   const int64_t row_blocks = (rows + 15) / 16, blocks = (cols + 127) / 128;
-  const int64_t want = (static_cast<int64_t>(sm_count()) * 16 + row_blocks - 1) / row_blocks;
+  const int64_t want = (static_cast<int64_t>(sm_count()) * 64 + row_blocks - 1) / row_blocks;
   const dim3 grid(static_cast<unsigned>(row_blocks), static_cast<unsigned>(want < blocks ? want : (blocks < 65535 ? blocks : 65535)));
 #define AB200_QROWS(T)                                                                                                            \
   quantize_rows_kernel<T><<<grid, 256, 0, stream>>>(static_cast<const T*>(x), ld_x, vec, static_cast<uint8_t*>(q), ld_q, scale,   \
@@ -541,7 +571,7 @@ int ab200_float8_product(const void* x, const float* x_scale, const void* w, con
   g.b_scale = w_scale; g.b_scale_group = w_scale_group_stride; g.b_scale_n = w_scale_stride_n; g.b_scale_k = w_scale_stride_k;
   p.a = x; p.a_pitch = ld_x;
   p.b = w; p.b_pitch = ld_w; p.b_group_pitch = w_group_stride; p.b_rows = g.N; p.b_cols = g.K;
-  const Tile t = pick_tile(rows, groups, N, p.allow_pair, 32);
+  const Tile t = pick_tile(kCosts8, N, p.allow_pair, ragged_row_tiles(rows, groups));
   set_last_path(AB200_PATH_TCGEN05);
   return launch_grouped_8(p, t.bn, t.pair, stream);
 }

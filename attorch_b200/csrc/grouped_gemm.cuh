@@ -114,8 +114,8 @@ struct GroupedCfg {
   static constexpr uint32_t MN_LAYOUT = MN_BASE32 ? ptx::kLayoutSw128Base32 : ptx::kLayoutSw128;
   static constexpr uint32_t MN_SBO = MN_BASE32 ? 512 : 1024;
   // 8-bit: 12 warps, the epilogue's two warpgroups (warps 4-11) take registers over from the first one: with
-  // 168 a thread (384 threads at launch) part of the 128 accumulators lived in local memory, and a stage took 3 us
-  // instead of 0.3.  256 * 224 + 128 * 56 = 384 * 168.
+  // 168 a thread (384 threads at launch) part of the 128 accumulators lived in local memory, and 8192 x 4096 x 4096
+  // took 425 us instead of 145.  256 * 224 + 128 * 56 = 384 * 168.
   static constexpr int kFirstEpilogueWarp = kScaled ? 4 : 2;
   static constexpr int kThreads = 32 * (kFirstEpilogueWarp + kEpilogueWarps);
   static constexpr int kEpilogueRegs = 224, kOtherRegs = 56;
@@ -661,19 +661,16 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
           if (!wait(acc_full_bar(d), (n_acc / Cfg::kAccs) & 1u, DEV_TIMEOUT_EPILOGUE)) { ok = false; break; }
           n_acc += Cfg::kSubs;
           ptx::tc_fence_after_sync();
-          // The accumulator is handed back before the last arithmetic.  A warp without rows only hands it back.  Two chunks
-          // are loaded together where they are all; of four, more than one at a time cost registers (spills: 197
-          // against 184 us at 8192 x 4096 x 4096).
-          constexpr int kTwo = kChunks == 2 ? 2 : 1;
+          // One chunk at a time, and none skipped where it has no rows: two at a time, or a load under a condition, made
+          // the compiler spill accumulators in this loop (8192 x 4096 x 4096: 197 and 184 us against 145).  The
+          // accumulator is handed back before the last arithmetic.
 #pragma unroll
-          for (int c0 = 0; c0 < kChunks; c0 += kTwo) {
-            uint32_t r[kTwo][32];
-#pragma unroll
-            for (int i = 0; i < kTwo; ++i)
-              if (chunk_at(c0 + i) < BN / 32 && row0 < t.row_end)
-                ptx::tmem_ld_32x32(tmem_base + lane_base + d * Cfg::SUB + (chunk_at(c0 + i) % (Cfg::SUB / 32)) * 32, r[i]);
+          for (int ci = 0; ci < kChunks; ++ci) {
+            if (BN < 64 && half != 0) break;               // the narrowest tile has one chunk
+            uint32_t r[32];
+            ptx::tmem_ld_32x32(tmem_base + lane_base + d * Cfg::SUB + (chunk_at(ci) % (Cfg::SUB / 32)) * 32, r);
             ptx::tmem_ld_wait();
-            if (c0 + kTwo >= kChunks) {
+            if (ci + 1 == kChunks) {
               ptx::tc_fence_before_sync();
               __syncwarp();
               if (lane == 0) {
@@ -682,18 +679,14 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
               }
             }
 #pragma unroll
-            for (int i = 0; i < kTwo; ++i)
-              if (chunk_at(c0 + i) < BN / 32 && row0 < t.row_end) {
-                float (&sum)[32] = acc[c0 + i];
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                  const float2 f = actm::fma2(make_float2(__uint_as_float(r[i][e]), __uint_as_float(r[i][e + 1])),
-                                              actm::both(sc), make_float2(sum[e], sum[e + 1]));
-                  sum[e] = f.x;
-                  sum[e + 1] = f.y;
-                }
-              }
+            for (int i = 0; i < 32; i += 2) {
+              const float2 f = actm::fma2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), actm::both(sc),
+                                          make_float2(acc[ci][i], acc[ci][i + 1]));
+              acc[ci][i] = f.x;
+              acc[ci][i + 1] = f.y;
+            }
           }
+          if (BN < 64 && half != 0 && lane == 0) ptx::mbar_arrive(acc_empty_bar(d));
         }
         if (!ok) break;
       } else if (k_blocks > 0) {

@@ -30,7 +30,7 @@ struct GroupedProblem {
 int encode_3d(CUtensorMap* map, int elt, const void* base, uint64_t inner, uint64_t rows, uint64_t outer, uint64_t pitch_bytes,
               uint64_t group_bytes, uint32_t box_inner, uint32_t box_rows, CUtensorMapSwizzle swizzle);
 
-// Families; bn in {32 (8-bit), 64, 128, 256}, pair only with bn = 256.
+// Families; bn in {32 (8-bit), 64, 128, 256 (not 8-bit)}, pairs of CTAs with bn = 256.
 int launch_grouped_forward_16(const GroupedProblem& p, int bn, bool pair, cudaStream_t stream);
 int launch_grouped_input_16(const GroupedProblem& p, int bn, bool pair, cudaStream_t stream);
 int launch_grouped_weight_16(const GroupedProblem& p, int bn, bool pair, cudaStream_t stream);

@@ -1,7 +1,8 @@
 // Top-k routing of tokens to experts, and the moves between token order and expert order.
 //
-// Selection: one warp a token holds the row of logits in registers (E <= 512: 16 a lane) as order-preserving
-// integers, and takes k times the maximum (redux over the warp) and the lowest index that has it.  -inf and
+// Selection: one warp a token holds the row of logits in registers (E <= 512: 16 consecutive ones a lane) as
+// order-preserving integers, and takes k times the maximum (redux over the lanes' own) from the first lane that has it;
+// only that lane looks at its registers again.  -inf and
 // masked rows are integer 0, which is never taken.
 // Plan: a stable counting sort of the (token, expert) pairs by expert.  A block counts its tokens per warp and
 // expert; with more than one block the counts go to memory and a second kernel adds up what lies before
@@ -56,26 +57,35 @@ template <int kRegs>
 __device__ __forceinline__ void select_token(const RouteArgs& a, int token, int lane, const float (&v)[kRegs], bool live,
                                              int& expert, float& weight) {
   uint32_t key[kRegs];
+  uint32_t own = 0u;                                                // the lane's largest
 #pragma unroll
-  for (int i = 0; i < kRegs; ++i) key[i] = live && i * 32 + lane < a.experts ? order_key(v[i]) : 0u;
+  for (int i = 0; i < kRegs; ++i) {
+    key[i] = live && lane * kRegs + i < a.experts ? order_key(v[i]) : 0u;
+    own = max(own, key[i]);
+  }
   uint32_t mine = 0u, largest = 0u;
   expert = -1;
   for (int j = 0; j < a.k; ++j) {
-    uint32_t best = 0u;
-#pragma unroll
-    for (int i = 0; i < kRegs; ++i) best = max(best, key[i]);
-    best = __reduce_max_sync(0xFFFFFFFFu, best);
+    const uint32_t best = __reduce_max_sync(0xFFFFFFFFu, own);
     if (best == 0u) break;                                          // nothing left to choose
-    uint32_t at = 0xFFFFFFFFu;
+    // Experts ascend over the lanes and within one: the first lane's first is the lowest index.
+    const int first = __ffs(__ballot_sync(0xFFFFFFFFu, own == best)) - 1;
+    int at = 0;
+    if (lane == first) {
 #pragma unroll
-    for (int i = kRegs - 1; i >= 0; --i)
-      if (key[i] == best) at = i * 32 + lane;
-    at = __reduce_min_sync(0xFFFFFFFFu, at);
+      for (int i = kRegs - 1; i >= 0; --i)
+        if (key[i] == best) at = i;
+      own = 0u;
 #pragma unroll
-    for (int i = 0; i < kRegs; ++i)
-      if (at == static_cast<uint32_t>(i * 32 + lane)) key[i] = 0u;
+      for (int i = 0; i < kRegs; ++i) {
+        if (i == at) key[i] = 0u;
+        own = max(own, key[i]);
+      }
+      at += lane * kRegs;
+    }
+    at = __shfl_sync(0xFFFFFFFFu, at, first);
     if (j == 0) largest = best;
-    if (lane == j) { expert = static_cast<int>(at); mine = best; }
+    if (lane == j) { expert = at; mine = best; }
   }
   const float top = largest == 0xFFFFFFFFu ? __uint_as_float(0x7FC00000u) : key_value(largest);
   float score = 0.0f, sum = 0.0f;
@@ -91,7 +101,7 @@ __device__ __forceinline__ void select_token(const RouteArgs& a, int token, int 
   } else {
 #pragma unroll
     for (int i = 0; i < kRegs; ++i)
-      if (i * 32 + lane < a.experts) sum += expf(v[i] - top);
+      if (lane * kRegs + i < a.experts) sum += expf(v[i] - top);
     sum = warp_sum(sum);
     weight = score / sum;
   }
@@ -176,7 +186,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_select_kernel(const Ro
   auto load = [&](int t, float (&v)[kRegs]) {
 #pragma unroll
     for (int i = 0; i < kRegs; ++i)
-      v[i] = (t < t1 && i * 32 + lane < a.experts) ? load_as_f32(a.logits, a.dtype, t * a.ld + i * 32 + lane) : -INFINITY;
+      v[i] = (t < t1 && lane * kRegs + i < a.experts) ? load_as_f32(a.logits, a.dtype, t * a.ld + lane * kRegs + i) : -INFINITY;
   };
   float next[kRegs];
   load(t0, next);
@@ -236,16 +246,21 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_place_kernel(const Rou
     }
     __syncwarp();
   }
-  // Integer sums in shared memory: exact in any order.
-  const int mine = blockIdx.x * E, n = gridDim.x * E;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    const int c = a.counts[i];
-    if (c != 0) {
-      const int e = i % E;
-      atomicAdd(&total[e], c);
-      if (i < mine) atomicAdd(&before[e], c);
+  // Every thread adds up one expert over every parts-th block; the parts meet in shared memory (integers: exact in any
+  // order).
+  const int parts = max(1, static_cast<int>(blockDim.x) / E);
+  const int part = threadIdx.x / E;
+  if (part < parts) {
+    const int e = threadIdx.x - part * E;
+    int sum = 0, lower = 0;
+#pragma unroll 8
+    for (int b = part; b < static_cast<int>(gridDim.x); b += parts) {
+      const int c = a.counts[static_cast<long long>(b) * E + e];
+      sum += c;
+      if (b < static_cast<int>(blockIdx.x)) lower += c;
     }
+    atomicAdd(&total[e], sum);
+    atomicAdd(&before[e], lower);
   }
   __syncthreads();
   for (int e = threadIdx.x; e < E; e += blockDim.x) {
@@ -375,8 +390,10 @@ struct RowUnit {
   alignas(sizeof(T) * kVec) T v[kVec];
 };
 
-// y[t] = sum_j w[t, j] rows[token_row[t, j]] (without weights: the plain sum), in fp32, j ascending.
-template <class T, int kVec>
+// y[t] = sum_j w[t, j] rows[token_row[t, j]] (without weights: the plain sum), in fp32, j ascending.  Where a token's
+// rows lie is looked up once (kAtOnce at a time), not per unit, and the loads of all of them are issued before the
+// first sum, without a condition: an absent row reads row 0 and is left out of the sum.
+template <class T, int kVec, int kAtOnce>
 __global__ void __launch_bounds__(256)
 combine_kernel(const T* __restrict__ rows, long long ld_rows, const int* __restrict__ token_row,
                const float* __restrict__ weights, T* __restrict__ y, long long ld_y, int tokens, int k, int num_rows, int units) {
@@ -384,28 +401,33 @@ combine_kernel(const T* __restrict__ rows, long long ld_rows, const int* __restr
   for (int t = blockIdx.x * blockDim.y + threadIdx.y; t < tokens; t += gridDim.x * blockDim.y) {
     const int* at = token_row + static_cast<long long>(t) * k;
     const float* wt = weights == nullptr ? nullptr : weights + static_cast<long long>(t) * k;
+    auto look_up = [&](int j0, int (&r)[kAtOnce], float (&w)[kAtOnce]) {
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        r[j] = j0 + j < k ? __ldg(at + j0 + j) : -1;
+        if (r[j] >= num_rows) r[j] = -1;
+        w[j] = wt == nullptr || j0 + j >= k ? 1.0f : __ldg(wt + j0 + j);
+      }
+    };
+    int r[kAtOnce];
+    float w[kAtOnce];
+    look_up(0, r, w);
     for (int u = threadIdx.x; u < units; u += blockDim.x) {
       float acc[kVec];
 #pragma unroll
       for (int i = 0; i < kVec; ++i) acc[i] = 0.0f;
-      for (int j0 = 0; j0 < k; j0 += 4) {
-        U in[4];
-        float w[4];
-        bool live[4];
+      for (int j0 = 0; j0 < k; j0 += kAtOnce) {
+        if (k > kAtOnce) look_up(j0, r, w);
+        U in[kAtOnce];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = j0 + j < k ? __ldg(at + j0 + j) : -1;
-          live[j] = r >= 0 && r < num_rows;
-          if (live[j]) {
-            in[j] = *reinterpret_cast<const U*>(rows + r * ld_rows + static_cast<long long>(u) * kVec);
-            w[j] = wt == nullptr ? 1.0f : __ldg(wt + j0 + j);
-          }
-        }
+        for (int j = 0; j < kAtOnce; ++j)
+          in[j] = *reinterpret_cast<const U*>(rows + max(r[j], 0) * ld_rows + static_cast<long long>(u) * kVec);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (live[j]) {
+        for (int j = 0; j < kAtOnce; ++j)
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) acc[i] = fmaf(w[j], to_f32<T>(in[j].v[i]), acc[i]);
+          for (int i = 0; i < kVec; ++i) {
+            const float sum = fmaf(w[j], to_f32<T>(in[j].v[i]), acc[i]);
+            acc[i] = r[j] >= 0 ? sum : acc[i];
           }
       }
       U out;
