@@ -26,5 +26,12 @@ def status_of(device: torch.device, stream: int) -> int:
     """Address of the status word of a stream of ``device``, which is current (see ``check_status``)."""
     entry = _scratch.get((device.index, stream))
     if entry is None:
+        if torch.cuda.is_current_stream_capturing():
+            # Made inside the capture the word would be zeroed by the graph's replays only, and ``check_status`` before the
+            # first of them would read whatever is there.  Any other stream's word of the device serves: it is written
+            # by a wait that ran out and by nothing else.
+            for (index, _), other in _scratch.items():
+                if index == device.index:
+                    return other['status'].data_ptr()
         entry = _stream_scratch(device)
     return entry['status'].data_ptr()

@@ -50,7 +50,8 @@ namespace {
 
 bool valid_dtype(int dt) { return dt == DT_F32 || dt == DT_F16 || dt == DT_BF16; }
 bool valid_act(int act) { return act >= 0 && act < ACT_COUNT; }
-bool fits_int(int64_t v) { return v >= 0 && v < (1ll << 31); }
+// Counts that kernels add tile and grid sizes to in 32 bits.
+bool fits_int(int64_t v) { return v >= 0 && v < (1ll << 31) - (1ll << 20); }
 bool aligned16(const void* p, int64_t ld, int elt) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * elt % 16 == 0; }
 int launched(int n = 1) {
   if (cudaGetLastError() != cudaSuccess) return ERR_LAUNCH;

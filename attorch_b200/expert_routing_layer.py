@@ -15,7 +15,8 @@ from torch import Tensor, nn
 
 from . import _lib
 from ._launch import on, status_of, stream_of
-from .linear_layer import (Linear, _as_operand, _cached_size, _dtype_id, _flags_for, _ptr, _require_cuda,
+from .grouped_linear_layer import _pitch, _rows_operand
+from .linear_layer import (Linear, _cached_size, _dtype_id, _flags_for, _ptr, _require_cuda,
                            get_output_dtype)
 
 MAX_EXPERTS, MAX_TOP_K = 512, 32
@@ -44,10 +45,6 @@ def _inner_unit(tensor: Tensor) -> Tensor:
     if (cols <= 1 or tensor.stride(1) == 1) and (rows <= 1 or tensor.stride(0) >= cols):
         return tensor
     return tensor.contiguous()
-
-
-def _pitch(tensor: Tensor) -> int:
-    return tensor.stride(0) if tensor.shape[0] > 1 else tensor.shape[1]
 
 
 _SCORE_FUNCS = {'softmax': 0, 'sigmoid': 1}
@@ -271,8 +268,8 @@ class GateAutoGrad(torch.autograd.Function):
         lib = _lib.load()
         with on(input.device):
             stream = stream_of(input.device)
-            x_op = _inner_unit(_as_operand(input, dtype, stream))
-            w_op = _inner_unit(_as_operand(weight, dtype, stream))
+            x_op = _rows_operand(input, dtype, stream)
+            w_op = _rows_operand(weight, dtype, stream)
             output = torch.empty((rows, experts), dtype=dtype, device=input.device)
             _lib.check(lib.ab200_grouped_linear_forward(
                 _ptr(x_op), _ptr(w_op), None, None, None, _ptr(output), rows, 1, in_dim, experts, _pitch(x_op), 0, _pitch(w_op),
@@ -293,7 +290,7 @@ class GateAutoGrad(torch.autograd.Function):
         with on(device):
             stream = stream_of(device)
             status = status_of(device, stream)
-            dy = _inner_unit(_as_operand(output_grad, dtype, stream))
+            dy = _rows_operand(output_grad, dtype, stream)
             dt = _dtype_id(dtype)
 
             def scratch(*shape: int) -> Tuple[Optional[Tensor], int]:

@@ -21,9 +21,8 @@ from torch import Tensor, nn
 from . import _lib
 from ._launch import on, status_of, stream_of
 from .acts import act_id, parse_act_func
-from .grouped_linear_layer import MAX_GROUPS, GroupedLinear, _check_offsets, _pitch
-from .linear_layer import (Linear, _as_operand, _cached_size, _dtype_id, _flags_for, _ptr, _require_cuda,
-                           _workspace, get_output_dtype)
+from .grouped_linear_layer import MAX_GROUPS, GroupedLinear, _check_offsets, _pitch, _rows_operand
+from .linear_layer import Linear, _cached_size, _dtype_id, _flags_for, _ptr, _require_cuda, get_output_dtype
 
 BLOCK = 128
 
@@ -210,9 +209,7 @@ class Float8LinearAutoGrad(torch.autograd.Function):
         out_dtype = get_output_dtype(input.dtype)
         with on(input.device):
             stream = stream_of(input.device)
-            x_op = _as_operand(flat, out_dtype, stream)
-            if x_op.shape[1] > 1 and x_op.stride(1) != 1 or (rows > 1 and x_op.stride(0) < in_dim):
-                x_op = x_op.contiguous()
+            x_op = _rows_operand(flat, out_dtype, stream)
             output = torch.empty((rows, out_dim), dtype=out_dtype, device=input.device)
             wq = scale = slope = None
             if output.numel():
@@ -243,22 +240,21 @@ class Float8LinearAutoGrad(torch.autograd.Function):
             stream = stream_of(device)
             status = status_of(device, stream)
             dt = _dtype_id(dtype)
-            dy = _as_operand(output_grad.reshape(rows, out_dim), dtype, stream)
-            if (out_dim > 1 and dy.stride(1) != 1) or (rows > 1 and dy.stride(0) < out_dim):
-                dy = dy.contiguous()
+            dy = _rows_operand(output_grad.reshape(rows, out_dim), dtype, stream)
             dz = dy
             if ctx.needs[2]:
                 bias_grad = torch.empty(out_dim, dtype=ctx.dtypes[2], device=device)
             if (slope is not None or ctx.needs[2]) and out_dim:
                 if slope is not None:
-                    dz = torch.empty((rows, out_dim), dtype=dtype, device=device)
+                    unit = 16 // dtype.itemsize
+                    dz = torch.empty((rows, -(-out_dim // unit) * unit), dtype=dtype, device=device)[:, :out_dim]
                 ws_bytes = _cached_size('ab200_act_backward_workspace_bytes', rows, out_dim) if ctx.needs[2] else 0
                 workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
                 act = _lib.ACT_NONE if slope is None else (
                     _lib.ACT_SAVED_DERIVATIVE if slope.dtype is dtype else _lib.ACT_SAVED_DERIVATIVE_F16)
                 _lib.check(lib.ab200_act_backward(
                     _ptr(dy), _ptr(slope), _ptr(dz) if slope is not None else None, _ptr(bias_grad), rows, out_dim, _pitch(dy),
-                    out_dim, out_dim, dt, _dtype_id(bias_grad.dtype) if bias_grad is not None else 0, act, 0.0, _ptr(workspace),
+                    out_dim, _pitch(dz), dt, _dtype_id(bias_grad.dtype) if bias_grad is not None else 0, act, 0.0, _ptr(workspace),
                     ws_bytes, stream), 'ab200_act_backward')
             if ctx.needs[1]:
                 weight_grad = torch.empty((in_dim, out_dim), dtype=ctx.dtypes[1], device=device)
@@ -297,8 +293,8 @@ class Float8Linear(Linear):
     def __init__(self, in_features: int, out_features: int, bias: bool = True, act_func: Optional[str] = None,
                  device='cuda', dtype: torch.dtype = torch.float32) -> None:
         super().__init__(in_features, out_features, bias, act_func, device, dtype)
-        self.register_buffer('weight_float8', None, persistent=False)
-        self.register_buffer('weight_scale', None, persistent=False)
+        self.register_buffer('weight_float8', None)
+        self.register_buffer('weight_scale', None)
 
     @classmethod
     def from_linear(cls, linear: Linear) -> 'Float8Linear':
@@ -318,6 +314,9 @@ class Float8Linear(Linear):
         return self
 
     def forward(self, input: Tensor, residual: Optional[Tensor] = None) -> Tensor:
+        if self.weight_grad_out is not None or self.grad_ready is not None or self.defer_input_grad is not None:
+            raise RuntimeError('Float8Linear does not write its gradients into a data-parallel bucket; use Linear, or reduce '
+                               '.grad after backward.')
         if self.weight is None:
             output = float8_linear(input, self.weight_float8, self.weight_scale, self.bias, self.act_func)
         else:

@@ -24,17 +24,27 @@ from .linear_layer import _cached_size, _dtype_id, _flags_for, _ptr, _require_cu
 MAX_GROUPS = 512
 
 
+def _pitch(tensor: Tensor) -> int:
+    """Row pitch in elements (the stride of a single row may mean nothing)."""
+    rows, cols = tensor.shape
+    return tensor.stride(0) if rows > 1 or tensor.stride(0) >= cols else cols
+
+
 def _rows_operand(tensor: Tensor, dtype: torch.dtype, stream: int) -> Tensor:
     """
-    A 2-D operand of ``dtype`` with unit inner stride that TMA can address where a copy can make it so:
-    the tensor itself, or a contiguous converted copy.
+    A 2-D operand of ``dtype`` that TMA can address (unit inner stride, base and row pitch on 16-byte boundaries): the
+    tensor itself, or a converted copy, whose rows are padded where their length is no multiple of 16 bytes.  Such a copy
+    costs one pass over the operand; the CUDA-core kernel it avoids was up to 10 times slower than the product.
     """
     rows, cols = tensor.shape
-    elt = dtype.itemsize
+    unit = 16 // dtype.itemsize
     if tensor.dtype is dtype and (cols <= 1 or tensor.stride(1) == 1):
-        pitch = tensor.stride(0) if rows > 1 else cols
-        if pitch >= cols and ((pitch * elt) % 16 == 0 and tensor.data_ptr() % 16 == 0 or (cols * elt) % 16 != 0):
+        pitch = _pitch(tensor)
+        if pitch >= cols and pitch % unit == 0 and tensor.data_ptr() % 16 == 0:
             return tensor
+    if cols % unit:
+        out = torch.empty((rows, -(-cols // unit) * unit), dtype=dtype, device=tensor.device)[:, :cols]
+        return out.copy_(tensor)
     out = torch.empty((rows, cols), dtype=dtype, device=tensor.device)
     if out.numel():
         _lib.check(_lib.load().ab200_cast_2d(tensor.data_ptr(), out.data_ptr(), rows, cols, tensor.stride(0), tensor.stride(1),
@@ -42,23 +52,18 @@ def _rows_operand(tensor: Tensor, dtype: torch.dtype, stream: int) -> Tensor:
     return out
 
 
-def _pitch(tensor: Tensor) -> int:
-    """Row pitch in elements (the stride of a single row means nothing)."""
-    return tensor.stride(0) if tensor.shape[0] > 1 else tensor.shape[1]
-
-
 def _stack_operand(weight: Tensor, dtype: torch.dtype, stream: int) -> Tensor:
-    """A stack of matrices of ``dtype`` with unit inner stride and matrices a whole number of rows apart."""
-    if weight.dtype is dtype and weight.is_contiguous():
-        return weight
+    """The same for a stack of matrices, which also lie a whole number of rows apart."""
     groups, rows, cols = weight.shape
-    if weight.dtype is dtype and weight.stride(2) == 1 and weight.stride(1) >= cols and \
-            weight.stride(0) >= rows * weight.stride(1) and weight.stride(0) % weight.stride(1) == 0:
+    unit = 16 // dtype.itemsize
+    if weight.dtype is dtype and (cols <= 1 or weight.stride(2) == 1) and weight.stride(1) >= max(cols, 1) and \
+            weight.stride(1) % unit == 0 and weight.data_ptr() % 16 == 0 and \
+            (groups == 1 or (weight.stride(0) >= rows * weight.stride(1) and weight.stride(0) % weight.stride(1) == 0)):
         return weight
-    flat = weight if weight.is_contiguous() else weight.contiguous()
-    if flat.dtype is dtype:
-        return flat
-    return _rows_operand(flat.view(groups * rows, cols), dtype, stream).view(groups, rows, cols)
+    if cols % unit or not weight.is_contiguous():
+        out = torch.empty((groups, rows, -(-cols // unit) * unit), dtype=dtype, device=weight.device)[..., :cols]
+        return out.copy_(weight)
+    return _rows_operand(weight.view(groups * rows, cols), dtype, stream).view(groups, rows, cols)
 
 
 def _check_offsets(offsets: Tensor, groups: int, input: Tensor) -> Tensor:
@@ -144,7 +149,8 @@ class GroupedLinearAutoGrad(torch.autograd.Function):
             dz = dy
             if slope is not None or ctx.needs[2]:
                 if slope is not None:
-                    dz = torch.empty((rows, out_dim), dtype=dtype, device=device)
+                    unit = 16 // dtype.itemsize
+                    dz = torch.empty((rows, -(-out_dim // unit) * unit), dtype=dtype, device=device)[:, :out_dim]
                 ws_bytes = 0
                 workspace = None
                 if ctx.needs[2]:
@@ -155,7 +161,7 @@ class GroupedLinearAutoGrad(torch.autograd.Function):
                     _lib.ACT_SAVED_DERIVATIVE if slope.dtype is dtype else _lib.ACT_SAVED_DERIVATIVE_F16)
                 _lib.check(lib.ab200_grouped_act_backward(
                     _ptr(dy), _ptr(slope), _ptr(dz) if slope is not None else None, _ptr(bias_grad), _ptr(offsets), rows, groups,
-                    out_dim, _pitch(dy), out_dim, out_dim, dt, _dtype_id(bias_grad.dtype) if bias_grad is not None else 0, act, 0.0,
+                    out_dim, _pitch(dy), out_dim, _pitch(dz), dt, _dtype_id(bias_grad.dtype) if bias_grad is not None else 0, act, 0.0,
                     _ptr(workspace), ws_bytes, stream), 'ab200_grouped_act_backward')
             if ctx.needs[1]:
                 weight_grad = torch.empty((groups, in_dim, out_dim), dtype=ctx.dtypes[1], device=device)

@@ -206,6 +206,11 @@ def test_layers():
         assert torch.equal(layer(x, residual=expected), expected + expected)
     with pytest.raises(RuntimeError, match='no gradient'):
         layer(x.clone().requires_grad_())
+    assert set(layer.state_dict()) == {'weight_float8', 'weight_scale', 'bias'}       # a frozen layer can be saved
+    bucketed = attorch.Float8Linear.from_linear(linear)
+    bucketed.weight_grad_out = torch.empty_like(linear.weight)
+    with pytest.raises(RuntimeError, match='bucket'):
+        bucketed(x)
     grouped = attorch.GroupedLinear(3, 128, 256, act_func='silu', dtype=torch.bfloat16)
     eight = attorch.Float8GroupedLinear.from_grouped(grouped)
     rows = torch.randn(50, 128, device='cuda').bfloat16()

@@ -270,3 +270,46 @@ def test_block_step_in_a_graph():
             # The gate's weight gradient is Linear's: its pieces are added in any order, then rounded to bf16.
             assert torch.equal(a, e) or (name == 'router.gate.weight' and relative_error(a, e) <= 2.0 ** -8), name
     attorch.check_status()
+
+
+def test_first_call_of_a_stream_inside_a_capture():
+    """The status word of a stream whose first call is captured is valid before the graph has run."""
+    block = attorch.MixtureOfExperts(32, 32, 4, 2, 'relu', dtype=torch.bfloat16)
+    x = torch.randn(20, 32, device='cuda').bfloat16()
+    with torch.no_grad():
+        expected = block(x)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+            y = block(x)
+        attorch.check_status()
+        graph.replay()
+        torch.cuda.synchronize()
+    assert torch.equal(y, expected)
+    attorch.check_status()
+
+
+def test_two_graphs_of_one_stream_replayed_together():
+    """Graphs captured on one stream share no workspace: replayed at once on two, both give their own results."""
+    block = attorch.MixtureOfExperts(64, 128, 8, 2, 'silu', dtype=torch.bfloat16)
+    xs = [torch.randn(600, 64, device='cuda').bfloat16() for _ in range(2)]
+    stream = torch.cuda.Stream()
+    graphs, outs = [], []
+    with torch.no_grad():
+        for x in xs:
+            block(x)
+        torch.cuda.synchronize()
+        for x in xs:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                outs.append(block(x))
+            graphs.append(graph)
+        replay = [torch.cuda.Stream(), torch.cuda.Stream()]
+        for _ in range(20):
+            for graph, s in zip(graphs, replay):
+                with torch.cuda.stream(s):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(xs, outs):
+            assert torch.equal(y, block(x))
+    attorch.check_status()
