@@ -98,6 +98,7 @@ Tile pick_tile(const TileCost (&costs)[kCount], int64_t N, bool allow_pair, F&& 
 auto ragged_row_tiles(int64_t rows, int64_t groups) {
   const int64_t used = groups < rows ? groups : rows;
   return [=](int tile_m) {
+    if (groups == 1) return (rows + tile_m - 1) / tile_m;
     const int64_t tiles = rows / tile_m + (used + 1) / 2;
     return tiles > used ? tiles : used;
   };
@@ -504,13 +505,17 @@ int ab200_float8_quantize_rows(const void* x, void* q, float* scale, int64_t row
   if (rows == 0 || cols == 0) return OK;
   if (!x || !q || !scale) return ERR_NULL_POINTER;
   if (ld_x < cols || ld_q < cols || ld_scale < rows || !aligned16(q, ld_q, 1)) return ERR_BAD_STRIDE;
-  const bool vec = aligned16(x, ld_x, dtype_size(dtype));
+  const bool vec = cols % 8 == 0 && aligned16(x, ld_x, dtype_size(dtype));
   const int64_t row_blocks = (rows + 15) / 16, blocks = (cols + 127) / 128;
-  const int64_t want = (static_cast<int64_t>(sm_count()) * 64 + row_blocks - 1) / row_blocks;
-  const dim3 grid(static_cast<unsigned>(row_blocks), static_cast<unsigned>(want < blocks ? want : (blocks < 65535 ? blocks : 65535)));
+  const int64_t steps = vec ? (blocks + 1) / 2 : blocks;
+  const dim3 grid(static_cast<unsigned>(row_blocks), static_cast<unsigned>(steps < 65535 ? steps : 65535));
 #define AB200_QROWS(T)                                                                                                            \
-  quantize_rows_kernel<T><<<grid, 256, 0, stream>>>(static_cast<const T*>(x), ld_x, vec, static_cast<uint8_t*>(q), ld_q, scale,   \
-                                                    ld_scale, static_cast<int>(rows), static_cast<int>(cols))
+  do {                                                                                                                            \
+    if (vec) quantize_rows_kernel<T, true><<<grid, 256, 0, stream>>>(static_cast<const T*>(x), ld_x, static_cast<uint8_t*>(q),    \
+        ld_q, scale, ld_scale, static_cast<int>(rows), static_cast<int>(cols));                                                   \
+    else quantize_rows_kernel<T, false><<<grid, 256, 0, stream>>>(static_cast<const T*>(x), ld_x, static_cast<uint8_t*>(q),       \
+        ld_q, scale, ld_scale, static_cast<int>(rows), static_cast<int>(cols));                                                   \
+  } while (0)
   if (dtype == DT_F32) AB200_QROWS(float);
   else if (dtype == DT_F16) AB200_QROWS(__half);
   else AB200_QROWS(__nv_bfloat16);

@@ -60,26 +60,50 @@ __device__ __forceinline__ uint32_t abs_max8(const float (&v)[8]) {
 // x [rows, cols] -> q [rows, pitch] e4m3 (columns up to the next multiple of 16 are zero), scale
 // [ceil(cols / 128)][scale_ld].  Half a warp takes 128 elements of a row (8 a lane, 16-byte loads for 2-byte
 // types), the 16 half-warps of a block 16 rows, so that the scales of a column of blocks are written
-// side by side.  Bound by HBM: 3 bytes an element.
-template <class T>
+// side by side.  Bound by HBM: 3 bytes an element.  kVec: rows are 16-byte aligned and whole units of 8 columns; then
+// kAtOnce blocks of a row are in flight at a time.
+template <class T, bool kVec>
 __global__ void __launch_bounds__(256)
-quantize_rows_kernel(const T* __restrict__ x, long long ld, bool vec, uint8_t* __restrict__ q, long long pitch,
+quantize_rows_kernel(const T* __restrict__ x, long long ld, uint8_t* __restrict__ q, long long pitch,
                      float* __restrict__ scale, long long scale_ld, int rows, int cols) {
+  constexpr int kAtOnce = kVec ? 2 : 1;
+  constexpr int kWords = static_cast<int>(sizeof(T)) / 2;
   const int lane = threadIdx.x & 15;
   const long long row = static_cast<long long>(blockIdx.x) * 16 + (threadIdx.x >> 4);
   const int blocks = (cols + 127) / 128;
-  for (int b = blockIdx.y; b < blocks; b += gridDim.y) {
-    const int col = b * 128 + lane * 8;
-    float v[8] = {};
-    if (row < rows && col < cols) load8<T>(x + row * ld + col, vec, cols - col, v);
-    uint32_t amax = abs_max8(v);
+  for (int b0 = blockIdx.y * kAtOnce; b0 < blocks; b0 += gridDim.y * kAtOnce) {
+    [[maybe_unused]] uint4 in[kAtOnce][kWords];
+    if constexpr (kVec) {
 #pragma unroll
-    for (int d = 8; d > 0; d >>= 1) amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
-    float s, inverse;
-    block_scale(amax, s, inverse);
-    if (row < rows) {
-      if (col < pitch) *reinterpret_cast<uint2*>(q + row * pitch + col) = to_e4m3x8(v, inverse);
-      if (lane == 0) scale[b * scale_ld + row] = s;
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int col = (b0 + i) * 128 + lane * 8;
+        const bool live = row < rows && col < cols;
+#pragma unroll
+        for (int w = 0; w < kWords; ++w)
+          in[i][w] = live ? __ldg(reinterpret_cast<const uint4*>(x + row * ld + col) + w) : make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int b = b0 + i;
+      const int col = b * 128 + lane * 8;
+      float v[8];
+      if constexpr (kVec) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = to_f32<T>(reinterpret_cast<const T*>(in[i])[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = row < rows && col + j < cols ? to_f32<T>(x[row * ld + col + j]) : 0.0f;
+      }
+      uint32_t amax = abs_max8(v);
+#pragma unroll
+      for (int d = 8; d > 0; d >>= 1) amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
+      float s, inverse;
+      block_scale(amax, s, inverse);
+      if (row < rows && b < blocks) {
+        if (col < pitch) *reinterpret_cast<uint2*>(q + row * pitch + col) = to_e4m3x8(v, inverse);
+        if (lane == 0) scale[b * scale_ld + row] = s;
+      }
     }
   }
 }

@@ -26,11 +26,11 @@
 //
 // 8-bit operands (kScaled) carry one fp32 scale per row and 128 elements of K for A and per 128 x 128
 // block for B.  A stage is exactly 128 elements of K, so each stage's product over 128 columns is one partial
-// sum with one scale per row: the issuer gives every such part one of four accumulators of 128 columns, and the
-// epilogue warps add scale * partial into fp32 registers (128 accumulators a thread at BN = 256) while the
-// next parts multiply.  Per SM a part takes 256 clocks of MMA (128 x 128 x 128 at 8192 multiply-adds a clock)
-// against 128 clocks of tensor-memory reads and 64-128 of fp32 fma, so the scaling can hide; four
-// accumulators cover the way there and back (commit, wake-up, read, arrival: about 600 clocks).
+// sum with one scale per row: the two issuers give every such part one of four accumulators of up to 128 columns, and
+// the epilogue warps add scale * partial into fp32 registers (128 accumulators a thread at BN = 256) while the
+// next parts multiply.  Per SM a part of 128 columns takes 256 clocks of MMA (128 x 128 x 128 at 8192
+// multiply-adds a clock) and 145 of packed fp32 fma (2.26 a pair and scheduler, measured); four accumulators cover
+// most of the way there and back (commit, wake-up, read, arrival).  8192 x 4096 x 4096: 143 us; 118 without the scaling.
 #pragma once
 #include "gemm_tcgen05.cuh"
 
@@ -641,6 +641,28 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         for (int ci = 0; ci < kChunks; ++ci)
 #pragma unroll
           for (int i = 0; i < 32; ++i) acc[ci][i] = 0.0f;
+        if (row0 >= t.row_end) {
+          // No rows of this warp's (few rows, or a group's end): it only keeps the rings moving.
+          for (int kb = 0; kb < k_blocks; ++kb) {
+            const int ss = n_scale % Cfg::kScaleStages;
+            const uint32_t d = (n_acc + (Cfg::kSubs > 1 ? half : 0)) % Cfg::kAccs;
+            if (!wait(acc_full_bar(d), (n_acc / Cfg::kAccs) & 1u, DEV_TIMEOUT_EPILOGUE)) { ok = false; break; }
+            n_acc += Cfg::kSubs;
+            if (kb % Cfg::kScaleBlocks + 1 == Cfg::kScaleBlocks || kb + 1 == k_blocks) {
+              if (!wait(scale_full_bar(ss), (n_scale / Cfg::kScaleStages) & 1u, DEV_TIMEOUT_EPILOGUE)) { ok = false; break; }
+              ++n_scale;
+              __syncwarp();
+              if (lane == 0) ptx::mbar_arrive(scale_empty_bar(ss));
+            }
+            __syncwarp();                 // every lane has seen the phase before it can end
+            if (lane == 0) {
+              if constexpr (kPair) ptx::mbar_arrive_cluster_read(acc_empty_bar(d), 0);
+              else ptx::mbar_arrive(acc_empty_bar(d));
+            }
+          }
+          if (!ok) break;
+          continue;
+        }
         for (int kb = 0; kb < k_blocks && ok; ++kb) {
           const int ss = n_scale % Cfg::kScaleStages;
           const int in_stage = kb % Cfg::kScaleBlocks;

@@ -34,7 +34,8 @@ def _rows_operand(tensor: Tensor, dtype: torch.dtype, stream: int) -> Tensor:
     """
     A 2-D operand of ``dtype`` that TMA can address (unit inner stride, base and row pitch on 16-byte boundaries): the
     tensor itself, or a converted copy, whose rows are padded where their length is no multiple of 16 bytes.  Such a copy
-    costs one pass over the operand; the CUDA-core kernel it avoids was up to 10 times slower than the product.
+    costs one pass over the operand; on the CUDA-core kernel a step of 3000 rows through 8 experts of 1001 x 1003 took 963 us
+    instead of 244.
     """
     rows, cols = tensor.shape
     unit = 16 // dtype.itemsize

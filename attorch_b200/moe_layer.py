@@ -1,7 +1,7 @@
 """
 ``MixtureOfExperts``: the transformer block's MLP (examples/wikitext-2/gpt.py:30-37 of the reference) with a
-weight per expert: gate, dispatch, up-projection with its fused activation, down-projection, combine.  Seven
-launches for a forward pass of a few tokens, none of which the host waits for.
+weight per expert: gate, routing, dispatch, up-projection with its fused activation, down-projection, combine.  A
+forward pass of up to 256 tokens is six launches (seven when gated), none of which the host waits for.
 """
 
 from typing import Optional
