@@ -362,11 +362,11 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   ptx::tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
 
-  auto wait = [&](uint32_t bar, uint32_t parity, int code) -> bool {
+  auto wait = [&](uint32_t bar, uint32_t parity, int code, bool cluster = false) -> bool {
     uint32_t spins = 0;
     uint64_t t0 = 0;
-    // Only rows cleared by the other CTA of a pair (ragged reduction) are memory that a wait has to acquire from it.
-    while (!(kPair && Cfg::kRaggedK ? ptx::mbar_try_wait_cluster(bar, parity) : ptx::mbar_try_wait(bar, parity))) {
+    // cluster: the wait acquires memory that the other CTA of a pair wrote (rows it cleared in the ragged reduction).
+    while (!(cluster ? ptx::mbar_try_wait_cluster(bar, parity) : ptx::mbar_try_wait(bar, parity))) {
       if ((++spins & 0x3FFu) == 0) {
         if (*abort_flag) return false;
         const uint64_t now = ptx::globaltimer_ns();
@@ -515,7 +515,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
                 // The leader multiplies both CTAs' operands: the other one says that its own are ready.
                 if (cta == 1) {
                   if (lane == 0) ptx::mbar_arrive_cluster(full_bar(s), 0);
-                } else if (!issuer_wait(full_bar(s), ph)) { ok = false; break; }
+                } else if (!__all_sync(0xFFFFFFFFu, wait(full_bar(s), ph, DEV_TIMEOUT_MMA, true))) { ok = false; break; }
               } else if (lane == 0) {
                 ptx::mbar_arrive(full_bar(s));      // keeps the phases of the full barrier in step
               }
