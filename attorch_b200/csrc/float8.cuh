@@ -57,8 +57,8 @@ __device__ __forceinline__ uint32_t abs_max8(const float (&v)[8]) {
   return m;
 }
 
-// x [rows, cols] -> q [rows, pitch] e4m3 (columns up to the next multiple of 16 are zero), scale
-// [ceil(cols / 128)][scale_ld].  Half a warp takes 128 elements of a row (8 a lane, 16-byte loads for 2-byte
+// x [rows, cols] -> q [rows, pitch] e4m3 (bytes up to the next multiple of 8 columns are zero, none behind them is
+// written: the pitch may be that of a wider buffer), scale [ceil(cols / 128)][scale_ld].  Half a warp takes 128 elements of a row (8 a lane, 16-byte loads for 2-byte
 // types), the 16 half-warps of a block 16 rows, so that the scales of a column of blocks are written
 // side by side.  Bound by HBM: 3 bytes an element.  kVec: rows are 16-byte aligned and whole units of 8 columns; then
 // kAtOnce blocks of a row are in flight at a time.
@@ -101,7 +101,7 @@ quantize_rows_kernel(const T* __restrict__ x, long long ld, uint8_t* __restrict_
       float s, inverse;
       block_scale(amax, s, inverse);
       if (row < rows && b < blocks) {
-        if (col < pitch) *reinterpret_cast<uint2*>(q + row * pitch + col) = to_e4m3x8(v, inverse);
+        if (col < cols) *reinterpret_cast<uint2*>(q + row * pitch + col) = to_e4m3x8(v, inverse);
         if (lane == 0) scale[b * scale_ld + row] = s;
       }
     }
@@ -109,7 +109,7 @@ quantize_rows_kernel(const T* __restrict__ x, long long ld, uint8_t* __restrict_
 }
 
 // One 128 x 128 block of w [rows, cols] (stack of groups) -> e4m3 as stored (q, [rows, pitch]) and transposed
-// (q_t, [cols, pitch_t]), either may be NULL; scale[group][column block][row block].  A thread holds 8 x 8
+// (q_t, [cols, pitch_t]), either may be NULL, with zeros as above; scale[group][column block][row block].  A thread holds 8 x 8
 // elements; the transposed block passes through shared memory in 8-byte units whose place in a row is
 // rotated by the thread's column, so that neither side meets a bank twice.
 template <class T>
@@ -145,7 +145,7 @@ quantize_weight_kernel(const T* __restrict__ w, long long group_pitch, long long
   if (q != nullptr) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (row0 + i < rows && col0 < pitch) *reinterpret_cast<uint2*>(q + (group * rows + row0 + i) * pitch + col0) = to_e4m3x8(v[i], inverse);
+      if (row0 + i < rows && col0 < cols) *reinterpret_cast<uint2*>(q + (group * rows + row0 + i) * pitch + col0) = to_e4m3x8(v[i], inverse);
   }
   if (q_t != nullptr) {
 #pragma unroll
@@ -158,7 +158,7 @@ quantize_weight_kernel(const T* __restrict__ w, long long group_pitch, long long
     for (int j = 0; j < 8; ++j) {
       const int c = j * 16 + ty;                    // column of the block = row of the transposed one
       const int col = blockIdx.x * 128 + c, k = blockIdx.y * 128 + tx * 8;
-      if (col < cols && k < pitch_t) *reinterpret_cast<uint2*>(q_t + (group * cols + col) * pitch_t + k) = tile[c][tx ^ (c >> 3)];
+      if (col < cols && k < rows) *reinterpret_cast<uint2*>(q_t + (group * cols + col) * pitch_t + k) = tile[c][tx ^ (c >> 3)];
     }
   }
 }

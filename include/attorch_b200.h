@@ -555,7 +555,7 @@ int ab200_expert_combine_backward(const void* dy, const void* rows_in, const int
 /*
  * q = e4m3(x / s) with s the smallest power of two that keeps a block's largest magnitude within 448: blocks of
  * 1 x 128 elements.  x: [rows, cols] of `dtype`, pitch ld_x.  q: [rows, cols] bytes, pitch ld_q (a multiple of 16, base
- * 16-byte aligned; bytes up to the next multiple of 8 columns are written as zeros).  scale: [ceil(cols / 128)] rows of
+ * 16-byte aligned; bytes up to the next multiple of 8 columns are written as zeros, none behind them).  scale: [ceil(cols / 128)] rows of
  * pitch ld_scale >= rows.  A block of zeros has scale 1; one with an infinity or NaN becomes NaN.
  */
 int ab200_float8_quantize_rows(const void* x, void* q, float* scale, int64_t rows, int64_t cols, int64_t ld_x, int64_t ld_q,
@@ -563,7 +563,8 @@ int ab200_float8_quantize_rows(const void* x, void* q, float* scale, int64_t row
 
 /*
  * The same over blocks of 128 x 128 of a stack of matrices [rows, cols]: as stored (q, [groups, rows, cols], pitch ld_q)
- * and transposed (q_t, [groups, cols, rows], pitch ld_q_t); either may be NULL.  scale: dense
+ * and transposed (q_t, [groups, cols, rows], pitch ld_q_t); either may be NULL.  Zeros up to the next multiple of 8
+ * columns of each and nothing behind them, as above.  scale: dense
  * [groups, ceil(cols / 128), ceil(rows / 128)].
  */
 int ab200_float8_quantize_weight(const void* w, void* q, void* q_t, float* scale, int64_t groups, int64_t rows, int64_t cols,
