@@ -708,7 +708,10 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
               acc[ci][i + 1] = f.y;
             }
           }
-          if (BN < 64 && half != 0 && lane == 0) ptx::mbar_arrive(acc_empty_bar(d));
+          if (BN < 64 && half != 0) {
+            __syncwarp();                 // every lane has seen the phase before it can end
+            if (lane == 0) ptx::mbar_arrive(acc_empty_bar(d));
+          }
         }
         if (!ok) break;
       } else if (k_blocks > 0) {

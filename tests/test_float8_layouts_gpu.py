@@ -51,3 +51,23 @@ def test_quantized_weights_leave_a_wider_buffer_alone(k, n):
     check_bytes(q_t[:n], 16, k, 'transposed')
     a, b = (t.contiguous().view(torch.float8_e4m3fn).float() for t in (q[:k, 16:16 + n], q_t[:n, 16:16 + k]))
     assert torch.equal(a, b.T)
+
+
+@pytest.mark.parametrize('rows', [1, 33, 100])
+@pytest.mark.parametrize('k,n', [(16384, 64), (8192, 1000), (128, 96)])
+def test_narrow_products_repeat(rows, k, n):
+    """
+    Few columns: tiles of 32, whose upper four epilogue warps only hand the accumulators back.  Long reductions, many
+    times over: every phase of the four accumulators is waited for by all lanes before it can be reused.
+    """
+    import attorch_b200 as attorch
+    g = torch.Generator(device='cuda').manual_seed(rows)
+    keep = 2.0 / k ** 0.5
+    x = (torch.randint(-1, 2, (rows, k), generator=g, device='cuda') * (torch.rand(rows, k, generator=g, device='cuda') < keep)).bfloat16()
+    w = (torch.randint(-1, 2, (k, n), generator=g, device='cuda') * (torch.rand(k, n, generator=g, device='cuda') < keep)).bfloat16()
+    weight, scale = attorch.quantize_weight(w)
+    expected = x.double() @ w.double()
+    for _ in range(50):
+        y = attorch.float8_linear(x, weight, scale)
+    assert float(expected.abs().max()) <= 256 and torch.equal(y.double(), expected)
+    attorch.check_status()
