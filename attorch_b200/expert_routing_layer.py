@@ -137,8 +137,9 @@ def route(logits: Tensor, top_k: int, score_func: str = 'softmax', renormalize: 
 def _check_plan(routing: Routing, device: torch.device, tokens: Optional[int]) -> None:
     assert routing.token_row.ndim == 2 and routing.token_row.dtype is torch.int32 and routing.token_row.is_contiguous() and \
         routing.token_row.device == device, 'token_row must be a contiguous 2D int32 tensor on the device of the rows'
-    assert routing.offsets.dtype is torch.int32 and routing.offsets.is_contiguous() and routing.offsets.device == device, \
-        'offsets must be a contiguous int32 tensor on the device of the rows'
+    assert routing.offsets.ndim == 1 and routing.offsets.shape[0] >= 1 and routing.offsets.dtype is torch.int32 and \
+        routing.offsets.is_contiguous() and routing.offsets.device == device, \
+        'offsets must be a contiguous 1D int32 tensor with an end of the last expert, on the device of the rows'
     assert tokens is None or routing.token_row.shape[0] == tokens, \
         f'The routing has {routing.token_row.shape[0]} tokens, the input {tokens}'
 

@@ -1,0 +1,19 @@
+"""What the expert block's operators and the 8-bit products check on the host, before any address is taken."""
+
+import pytest
+import torch
+
+import attorch_b200 as attorch
+from attorch_b200 import expert_routing_layer as routing_layer
+
+CPU = torch.device('cpu')
+
+
+@pytest.mark.parametrize('offsets', [torch.zeros(0, dtype=torch.int32), torch.zeros(2, 2, dtype=torch.int32),
+                                     torch.tensor(3, dtype=torch.int32), torch.zeros(3), torch.zeros(6, dtype=torch.int32)[::2]])
+def test_plans_without_an_end_are_refused(offsets):
+    """The end of the last expert's rows is read from the last entry: there has to be one."""
+    plan = torch.zeros(4, 2, dtype=torch.int32)
+    with pytest.raises(AssertionError, match='offsets'):
+        routing_layer._check_plan(attorch.Routing(torch.zeros(4, 2), plan, offsets, plan.flatten(), plan), CPU, 4)
+    routing_layer._check_plan(attorch.Routing(torch.zeros(4, 2), plan, torch.zeros(1, dtype=torch.int32), plan.flatten(), plan), CPU, 4)
