@@ -261,6 +261,7 @@ class GateAutoGrad(torch.autograd.Function):
     def forward(ctx, input: Tensor, weight: Tensor) -> Tensor:
         assert input.ndim == 2 and input.shape[1] == weight.shape[0], \
             f'Incompatible input ({input.shape}) and weights ({weight.shape}) shape'
+        assert weight.device == input.device, f'The weights are on {weight.device}, the input on {input.device}'
         _require_cuda(input, 'input')
         _require_cuda(weight, 'weight')
         rows, in_dim = input.shape

@@ -17,3 +17,10 @@ def test_plans_without_an_end_are_refused(offsets):
     with pytest.raises(AssertionError, match='offsets'):
         routing_layer._check_plan(attorch.Routing(torch.zeros(4, 2), plan, offsets, plan.flatten(), plan), CPU, 4)
     routing_layer._check_plan(attorch.Routing(torch.zeros(4, 2), plan, torch.zeros(1, dtype=torch.int32), plan.flatten(), plan), CPU, 4)
+
+
+def test_gate_refuses_weights_of_another_device():
+    """The kernel gets both addresses on the input's device."""
+    router = attorch.Router(8, 4, 2, device='meta')
+    with pytest.raises(AssertionError, match='weights are on meta'):
+        router(torch.zeros(3, 8))
