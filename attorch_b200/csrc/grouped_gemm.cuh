@@ -260,18 +260,18 @@ __device__ __forceinline__ void store_slice(void* base, int dt, long long offset
     if (i < valid) store_from_f32(base, dt, offset + i, v[i]);
 }
 
-// act_fwd_grad over 8 elements at a time: v <- act(v), and put(first element, act' of the 8) at v rounded to dt.
+// act_fwd_grad over 8 elements at a time: v <- act(v), and put(first element, act' of the 8) at the fp32 v.
 template <class F>
-__device__ __forceinline__ void act_fwd_grad_slices(float (&v)[32], int act, float p, int dt, F&& put) {
+__device__ __forceinline__ void act_fwd_grad_slices(float (&v)[32], int act, float p, F&& put) {
   dispatch_act(act, [&]<int A>() {
 #pragma unroll
     for (int i0 = 0; i0 < 32; i0 += 8) {
       float g[8];
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
-        float z0 = v[i0 + i], z1 = v[i0 + i + 1], y0, y1;
-        round_through2(z0, z1, dt);
-        actm::fwd_grad2<A>(v[i0 + i], v[i0 + i + 1], z0, z1, p, y0, y1, g[i], g[i + 1]);
+        const float z0 = v[i0 + i], z1 = v[i0 + i + 1];
+        float y0, y1;
+        actm::fwd_grad2<A>(z0, z1, z0, z1, p, y0, y1, g[i], g[i + 1]);
         v[i0 + i] = y0;
         v[i0 + i + 1] = y1;
       }
@@ -780,19 +780,13 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
           }
           if (Cfg::kScaled && args.aux != nullptr && args.save_grad) {
             if (row_ok) {
-              act_fwd_grad_slices(v, args.act, args.act_param, odt, [&](int i0, const float (&g)[8]) {
+              act_fwd_grad_slices(v, args.act, args.act_param, [&](int i0, const float (&g)[8]) {
                 store_slice(args.aux, gdt, static_cast<long long>(row) * args.ld_aux + col0 + i0, g, valid - i0);
               });
             }
           } else if (args.aux != nullptr && args.save_grad) {
-            float zr[32], g[32];
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              zr[i] = v[i];
-              zr[i + 1] = v[i + 1];
-              round_through2(zr[i], zr[i + 1], odt);
-            }
-            act_fwd_grad(v, zr, g, args.act, args.act_param);
+            float g[32];
+            act_fwd_grad(v, v, g, args.act, args.act_param);        // act' at the fp32 Z: nothing rounds it first
             emit(&tmap_aux, args.aux, args.ld_aux, (args.tma_store & 2) != 0, g, gdt);
           } else {
             if (args.aux != nullptr) emit(&tmap_aux, args.aux, args.ld_aux, (args.tma_store & 2) != 0, v, odt);

@@ -91,8 +91,8 @@ __global__ void __launch_bounds__(256) grouped_any_kernel(const AnyGroupedArgs p
         if (g.bias != nullptr)
           v[0] += round_through(load_as_f32(g.bias, g.bias_dtype, static_cast<long long>(t.group) * g.N + n), g.out_dtype);
         if (g.aux != nullptr && g.save_grad) {
-          float zr[1] = {round_through(v[0], g.out_dtype)}, d[1];
-          act_fwd_grad(v, zr, d, g.act, g.act_param);
+          float d[1];
+          act_fwd_grad(v, v, d, g.act, g.act_param);
           store_from_f32(g.aux, g.grad_dtype, m * g.ld_aux + n, d[0]);
         } else {
           if (g.aux != nullptr) store_from_f32(g.aux, g.out_dtype, m * g.ld_aux + n, v[0]);

@@ -468,7 +468,8 @@ int ab200_layer_norm_backward(const void* dy, const void* x, const float* mean, 
  *   w        stack of [K, N] (the layout of Linear's weight), pitches w_group_stride and ld_w (elements)
  *   bias     dense [groups, N] of bias_dtype, or NULL
  *   pre_act  [rows, N] or NULL: the value before the activation, or act'(Z) with AB200_FLAG_SAVE_DERIVATIVE
- *            (and AB200_FLAG_DERIVATIVE_FP16), as ab200_linear_forward
+ *            (and AB200_FLAG_DERIVATIVE_FP16), as ab200_linear_forward, but at the fp32 Z: there is no form of
+ *            these operators elsewhere whose rounding of Z to `dtype` would have to be matched
  *   out      [rows, N] of `dtype`
  * fp32 operands are multiplied as TF32.  Operands that are not 16-byte aligned, or whose pitches are no multiples
  * of 16 bytes, run on a CUDA-core kernel.  status is required.  flags: AB200_FLAG_FORCE_GENERIC,

@@ -1,0 +1,61 @@
+"""
+Where the experts' and the 8-bit products round, and where they must not: act'(Z), the bias gradient, the gate's logits, what
+forward keeps for backward.
+"""
+
+import pytest
+import torch
+
+import attorch_b200 as attorch
+from attorch_b200 import _lib
+from tests.expert_helpers import act64, offsets_of
+
+pytestmark = pytest.mark.gpu
+
+
+def fractions(shape, steps, size, generator):
+    """Multiples of 1 / steps within +-size."""
+    return torch.randint(-size * steps, size * steps + 1, shape, generator=generator, device='cuda') / steps
+
+
+def kept_slope(y):
+    """What a call kept of act'(Z): its last saved tensor."""
+    return y.grad_fn.saved_tensors[3]
+
+
+@pytest.mark.parametrize('act', ['gelu', 'silu', 'sigmoid'])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize('rows,n,flags', [(70, 40, 0), (1500, 1032, 0), (70, 40, _lib.FLAG_FORCE_GENERIC), (70, 39, 0)])
+def test_derivative_is_taken_at_the_unrounded_value(act, dtype, rows, n, flags):
+    """
+    Z is a multiple of 2^-11 within +-4, exact in fp32 and not in 16 bits.  What is kept of act'(Z) is rounded to fp16 (half
+    a step: 2^-11 of it) and evaluated in fp32 (a few 1e-6); act' of a rounded Z would be off by up to 2^-9 |Z| |act''|.
+    """
+    g = torch.Generator(device='cuda').manual_seed(rows)
+    x = fractions((rows, 8), 16, 1, g).to(dtype)
+    w = fractions((2, 8, n), 64, 1, g).to(dtype) / 2
+    counts = [rows // 3, rows - rows // 3]
+    z64 = torch.cat([x[:counts[0]].double() @ w[0].double(), x[counts[0]:].double() @ w[1].double()])
+    previous = attorch.set_gemm_flags(flags)
+    try:
+        y = attorch.grouped_linear(x, offsets_of(counts), w.requires_grad_(), None, act)
+    finally:
+        attorch.set_gemm_flags(previous)
+    slope = act64(z64, act)[1]
+    assert kept_slope(y).dtype is torch.float16
+    assert ((kept_slope(y).double() - slope).abs() <= 2.0 ** -11 * slope.abs() + 4e-6).all()
+
+
+@pytest.mark.parametrize('act', ['gelu', 'silu'])
+@pytest.mark.parametrize('rows,n', [(70, 40), (1500, 2056)])
+def test_derivative_of_8_bit_products_is_taken_at_the_unrounded_value(act, rows, n):
+    """The same; multiples of 1/8 within +-1 (four significant bits at most) are held exactly by e4m3."""
+    g = torch.Generator(device='cuda').manual_seed(rows)
+    size = torch.exp2(-torch.randint(0, 5, (rows, 1), generator=g, device='cuda').float())
+    x = (fractions((rows, 24), 8, 1, g) * size).bfloat16()
+    w = (fractions((24, n), 8, 1, g) / 2).bfloat16()
+    z64 = x.double() @ w.double()
+    y = attorch.Float8LinearAutoGrad.apply(x, w.requires_grad_(), None, act)
+    slope = act64(z64, act)[1]
+    assert kept_slope(y).dtype is torch.float16
+    assert ((kept_slope(y).double() - slope).abs() <= 2.0 ** -11 * slope.abs() + 4e-6).all()
