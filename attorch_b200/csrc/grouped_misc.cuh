@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256) grouped_any_kernel(const AnyGroupedArgs p
 }
 
 // ------------------------------------------------------------------------------------------------
-// dZ = dY * act'(Z) over the rows of all groups, and the column sums of dZ per group.  A block takes
+// dZ = dY * act'(Z) over the rows of all groups, and the column sums of the unrounded dZ per group.  A block takes
 // kGroupedRows consecutive rows and 256 columns (32 threads of 8 columns, 8 row lanes).  Its rows meet
 // one or more groups; the sums of its rows of group e go to slot (block row + e) of `partial`: along
 // the rows either the block or the group advances, so no two (block, group) pairs share a slot, and
@@ -197,12 +197,12 @@ grouped_act_backward_kernel(const T* __restrict__ dy, long long ld_dy, const T* 
             else zz[i] = to_f32<T>(zin[u][i]);
           }
           act_grad_mul(g, zz, act, act_param);
-          alignas(16) T o[8];
-          pack8<T>(g, o);
           if (partial != nullptr) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum[i] += to_f32<T>(o[i]);      // what the weight gradient multiplies
+            for (int i = 0; i < 8; ++i) sum[i] += g[i];                 // in fp32: only dZ as it is stored is rounded
           }
+          alignas(16) T o[8];
+          pack8<T>(g, o);
           if (dz != nullptr) {
             if constexpr (kVec) {
 #pragma unroll

@@ -493,7 +493,7 @@ int ab200_grouped_linear_backward_weight(const void* x, const void* dz, const in
 /*
  * dZ = dY * act'(Z) on the rows of all experts, db[e] = sum of dZ over expert e's rows (dense [groups, N]); the
  * grouped form of ab200_act_backward, same arguments.  Rows of dz behind the last expert's are not written.
- * Sums are fp32 in a fixed order.
+ * Sums are fp32 in a fixed order, of dZ before it is rounded to `dtype`.
  */
 int ab200_grouped_act_backward(const void* dy, const void* z, void* dz, void* db, const int* offsets, int64_t rows, int64_t groups,
                                int64_t N, int64_t ld_dy, int64_t ld_z, int64_t ld_dz, int dtype, int db_dtype, int act,

@@ -59,3 +59,20 @@ def test_derivative_of_8_bit_products_is_taken_at_the_unrounded_value(act, rows,
     slope = act64(z64, act)[1]
     assert kept_slope(y).dtype is torch.float16
     assert ((kept_slope(y).double() - slope).abs() <= 2.0 ** -11 * slope.abs() + 4e-6).all()
+
+
+@pytest.mark.parametrize('n', [40, 39])
+@pytest.mark.parametrize('counts', [[256, 0, 64], [3, 1000]])
+def test_bias_gradient_sums_unrounded_values(counts, n):
+    """
+    dZ = 129/128 * 3/4 = 387/512 lies halfway between two bf16 numbers.  Its sum over a group's rows is a multiple of 1/512
+    below 2^11, exact in fp32; a sum of rounded values would be off by a 387th.
+    """
+    rows = sum(counts)
+    x = torch.ones(rows, 8, device='cuda', dtype=torch.bfloat16)
+    w = torch.full((len(counts), 8, n), -1.0, device='cuda', dtype=torch.bfloat16)
+    b = torch.zeros(len(counts), n, device='cuda', requires_grad=True)
+    y = attorch.grouped_linear(x, offsets_of(counts), w, b, 'leaky_relu_0.75')
+    db, = torch.autograd.grad(y, b, torch.full_like(y, 129 / 128))
+    expected = torch.tensor(counts, device='cuda')[:, None] * (387 / 512)
+    assert db.dtype is torch.float32 and torch.equal(db, expected.expand(-1, n))
