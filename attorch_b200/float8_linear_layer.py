@@ -21,7 +21,7 @@ from torch import Tensor, nn
 from . import _lib
 from ._launch import on, status_of, stream_of
 from .acts import act_id, parse_act_func
-from .grouped_linear_layer import MAX_GROUPS, GroupedLinear, _check_offsets, _pitch, _rows_operand
+from .grouped_linear_layer import MAX_GROUPS, GroupedLinear, _check_offsets, _kept_for_backward, _pitch, _rows_operand
 from .linear_layer import Linear, _cached_size, _dtype_id, _flags_for, _ptr, _require_cuda, get_output_dtype
 
 BLOCK = 128
@@ -211,27 +211,24 @@ class Float8LinearAutoGrad(torch.autograd.Function):
             stream = stream_of(input.device)
             x_op = _rows_operand(flat, out_dtype, stream)
             output = torch.empty((rows, out_dim), dtype=out_dtype, device=input.device)
-            wq = scale = slope = None
+            wq = scale = kept = None
+            ctx.backward_act = (_lib.ACT_NONE, 0.0)
             if output.numel():
                 xq, x_scale = _quantize_rows(x_op, stream)
                 wq, wq_t, scale = _quantize_weight(weight, ctx.needs[0], True, stream)
-                flags = 0
-                if name is not None and any(ctx.needs):
-                    fp16 = out_dtype is torch.bfloat16
-                    slope = torch.empty((rows, out_dim), dtype=torch.float16 if fp16 else out_dtype, device=input.device)
-                    flags = _lib.FLAG_SAVE_DERIVATIVE | (_lib.FLAG_DERIVATIVE_FP16 if fp16 else 0)
+                kept, flags, ctx.backward_act = _kept_for_backward(name, param, out_dtype, (rows, out_dim), input.device, any(ctx.needs))
                 bias_op = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-                _product(xq, x_scale, wq_t, scale, (0, scale.shape[1], 1), bias_op, None, slope, output, act_id(name),
+                _product(xq, x_scale, wq_t, scale, (0, scale.shape[1], 1), bias_op, None, kept, output, act_id(name),
                          0.0 if param is None else param, stream, flags)
         ctx.shapes = (input.shape, rows, in_dim, out_dim)
         ctx.dtypes = (input.dtype, weight.dtype, None if bias is None else bias.dtype)
         if any(ctx.needs):
-            ctx.save_for_backward(x_op if ctx.needs[1] else None, wq, scale, slope)
+            ctx.save_for_backward(x_op if ctx.needs[1] else None, wq, scale, kept)
         return output.view(*input.shape[:-1], out_dim)
 
     @staticmethod
     def backward(ctx, output_grad: Tensor) -> Tuple[Optional[Tensor], ...]:
-        x_op, wq, scale, slope = ctx.saved_tensors
+        x_op, wq, scale, kept = ctx.saved_tensors
         shape, rows, in_dim, out_dim = ctx.shapes
         device, dtype = output_grad.device, output_grad.dtype
         lib = _lib.load()
@@ -244,18 +241,16 @@ class Float8LinearAutoGrad(torch.autograd.Function):
             dz = dy
             if ctx.needs[2]:
                 bias_grad = torch.empty(out_dim, dtype=ctx.dtypes[2], device=device)
-            if (slope is not None or ctx.needs[2]) and out_dim:
-                if slope is not None:
+            if (kept is not None or ctx.needs[2]) and out_dim:
+                if kept is not None:
                     unit = 16 // dtype.itemsize
                     dz = torch.empty((rows, -(-out_dim // unit) * unit), dtype=dtype, device=device)[:, :out_dim]
                 ws_bytes = _cached_size('ab200_act_backward_workspace_bytes', rows, out_dim) if ctx.needs[2] else 0
                 workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
-                act = _lib.ACT_NONE if slope is None else (
-                    _lib.ACT_SAVED_DERIVATIVE if slope.dtype is dtype else _lib.ACT_SAVED_DERIVATIVE_F16)
                 _lib.check(lib.ab200_act_backward(
-                    _ptr(dy), _ptr(slope), _ptr(dz) if slope is not None else None, _ptr(bias_grad), rows, out_dim, _pitch(dy),
-                    out_dim, _pitch(dz), dt, _dtype_id(bias_grad.dtype) if bias_grad is not None else 0, act, 0.0, _ptr(workspace),
-                    ws_bytes, stream), 'ab200_act_backward')
+                    _ptr(dy), _ptr(kept), _ptr(dz) if kept is not None else None, _ptr(bias_grad), rows, out_dim, _pitch(dy),
+                    out_dim, _pitch(dz), dt, _dtype_id(bias_grad.dtype) if bias_grad is not None else 0, *ctx.backward_act,
+                    _ptr(workspace), ws_bytes, stream), 'ab200_act_backward')
             if ctx.needs[1]:
                 weight_grad = torch.empty((in_dim, out_dim), dtype=ctx.dtypes[1], device=device)
                 ws_bytes = _cached_size('ab200_gemm_workspace_bytes', in_dim, out_dim, rows)

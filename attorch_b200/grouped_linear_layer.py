@@ -17,6 +17,7 @@ import torch
 from torch import Tensor, nn
 
 from . import _lib
+from . import linear_layer as _layer
 from ._launch import on, status_of, stream_of
 from .acts import act_id, parse_act_func
 from .linear_layer import _cached_size, _dtype_id, _flags_for, _ptr, _require_cuda, get_output_dtype
@@ -90,9 +91,29 @@ def _check_operands(input: Tensor, weight: Tensor, bias: Optional[Tensor]) -> No
             assert tensor.device == input.device, f'{name} is on {tensor.device}, the input on {input.device}'
 
 
+def _kept_for_backward(name: Optional[str], param: Optional[float], dtype: torch.dtype, shape: Tuple[int, int],
+                       device: torch.device, needs_grad: bool):
+    """
+    What a forward call keeps of its activation, as ``set_save_derivative`` says: (the tensor or None, flags of the call, the
+    activation id and parameter that backward multiplies dY with).  act'(Z) in a bf16 layer is held as fp16, as
+    ``Linear`` holds it: the same size and three more bits; Z has the layer's type.
+    """
+    if name is None or not needs_grad:
+        return None, 0, (_lib.ACT_NONE, 0.0)
+    if not _layer._save_derivative:
+        return torch.empty(shape, dtype=dtype, device=device), 0, (act_id(name), 0.0 if param is None else param)
+    fp16 = dtype is torch.bfloat16
+    return (torch.empty(shape, dtype=torch.float16 if fp16 else dtype, device=device),
+            _lib.FLAG_SAVE_DERIVATIVE | (_lib.FLAG_DERIVATIVE_FP16 if fp16 else 0),
+            (_lib.ACT_SAVED_DERIVATIVE_F16 if fp16 else _lib.ACT_SAVED_DERIVATIVE, 0.0))
+
+
 def _forward(input: Tensor, offsets: Tensor, weight: Tensor, bias: Optional[Tensor], act_func: Optional[str],
              needs_grad: bool):
-    """(output, saved) where saved is what backward needs: operands, offsets, act'(Z)."""
+    """
+    (output, saved, backward_act) where saved is what backward needs: operands, offsets, and act'(Z) or Z; backward_act is the
+    activation id and parameter that turn the last of them into the factor of dY.
+    """
     _check_operands(input, weight, bias)
     name, param = parse_act_func(act_func)
     groups, in_dim, out_dim = weight.shape
@@ -107,19 +128,13 @@ def _forward(input: Tensor, offsets: Tensor, weight: Tensor, bias: Optional[Tens
         w_op = _stack_operand(weight, out_dtype, stream)
         bias_op = bias if bias is None or bias.is_contiguous() else bias.contiguous()
         output = torch.empty((rows, out_dim), dtype=out_dtype, device=input.device)
-        slope = None
-        flags = _flags_for(input.device)
-        if needs_grad and name is not None:
-            # act'(Z) instead of Z, in a bf16 layer as fp16, as Linear keeps it.
-            fp16 = out_dtype is torch.bfloat16
-            slope = torch.empty((rows, out_dim), dtype=torch.float16 if fp16 else out_dtype, device=input.device)
-            flags |= _lib.FLAG_SAVE_DERIVATIVE | (_lib.FLAG_DERIVATIVE_FP16 if fp16 else 0)
+        kept, keep_flags, backward_act = _kept_for_backward(name, param, out_dtype, (rows, out_dim), input.device, needs_grad)
         _lib.check(lib.ab200_grouped_linear_forward(
-            _ptr(x_op), _ptr(w_op), _ptr(bias_op), _ptr(offsets), _ptr(slope), _ptr(output), rows, groups, in_dim, out_dim,
+            _ptr(x_op), _ptr(w_op), _ptr(bias_op), _ptr(offsets), _ptr(kept), _ptr(output), rows, groups, in_dim, out_dim,
             _pitch(x_op), w_op.stride(0), w_op.stride(1), out_dim, out_dim, _dtype_id(out_dtype),
             _dtype_id(bias_op.dtype) if bias_op is not None else 0, act_id(name), 0.0 if param is None else param, status,
-            stream, flags), 'ab200_grouped_linear_forward')
-    return output, (x_op, w_op, offsets, slope), act_id(name)
+            stream, _flags_for(input.device) | keep_flags), 'ab200_grouped_linear_forward')
+    return output, (x_op, w_op, offsets, kept), backward_act
 
 
 class GroupedLinearAutoGrad(torch.autograd.Function):
@@ -128,7 +143,7 @@ class GroupedLinearAutoGrad(torch.autograd.Function):
     def forward(ctx, input: Tensor, offsets: Tensor, weight: Tensor, bias: Optional[Tensor] = None,
                 act_func: Optional[str] = None) -> Tensor:
         ctx.needs = (input.requires_grad, weight.requires_grad, bias is not None and bias.requires_grad)
-        output, saved, ctx.act = _forward(input, offsets, weight, bias, act_func, any(ctx.needs))
+        output, saved, ctx.backward_act = _forward(input, offsets, weight, bias, act_func, any(ctx.needs))
         ctx.dtypes = (input.dtype, weight.dtype, None if bias is None else bias.dtype)
         if any(ctx.needs):
             ctx.save_for_backward(*saved)
@@ -136,7 +151,7 @@ class GroupedLinearAutoGrad(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, output_grad: Tensor) -> Tuple[Optional[Tensor], ...]:
-        x_op, w_op, offsets, slope = ctx.saved_tensors
+        x_op, w_op, offsets, kept = ctx.saved_tensors
         groups, in_dim, out_dim = w_op.shape
         rows, device, dtype = x_op.shape[0], x_op.device, x_op.dtype
         dt = _dtype_id(dtype)
@@ -148,8 +163,8 @@ class GroupedLinearAutoGrad(torch.autograd.Function):
             flags = _flags_for(device)
             dy = _rows_operand(output_grad, dtype, stream)
             dz = dy
-            if slope is not None or ctx.needs[2]:
-                if slope is not None:
+            if kept is not None or ctx.needs[2]:
+                if kept is not None:
                     unit = 16 // dtype.itemsize
                     dz = torch.empty((rows, -(-out_dim // unit) * unit), dtype=dtype, device=device)[:, :out_dim]
                 ws_bytes = 0
@@ -158,12 +173,10 @@ class GroupedLinearAutoGrad(torch.autograd.Function):
                     bias_grad = torch.empty((groups, out_dim), dtype=ctx.dtypes[2], device=device)
                     ws_bytes = _cached_size('ab200_grouped_act_backward_workspace_bytes', rows, groups, out_dim)
                     workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
-                act = _lib.ACT_NONE if slope is None else (
-                    _lib.ACT_SAVED_DERIVATIVE if slope.dtype is dtype else _lib.ACT_SAVED_DERIVATIVE_F16)
                 _lib.check(lib.ab200_grouped_act_backward(
-                    _ptr(dy), _ptr(slope), _ptr(dz) if slope is not None else None, _ptr(bias_grad), _ptr(offsets), rows, groups,
-                    out_dim, _pitch(dy), out_dim, _pitch(dz), dt, _dtype_id(bias_grad.dtype) if bias_grad is not None else 0, act, 0.0,
-                    _ptr(workspace), ws_bytes, stream), 'ab200_grouped_act_backward')
+                    _ptr(dy), _ptr(kept), _ptr(dz) if kept is not None else None, _ptr(bias_grad), _ptr(offsets), rows, groups,
+                    out_dim, _pitch(dy), out_dim, _pitch(dz), dt, _dtype_id(bias_grad.dtype) if bias_grad is not None else 0,
+                    *ctx.backward_act, _ptr(workspace), ws_bytes, stream), 'ab200_grouped_act_backward')
             if ctx.needs[1]:
                 weight_grad = torch.empty((groups, in_dim, out_dim), dtype=ctx.dtypes[1], device=device)
                 _lib.check(lib.ab200_grouped_linear_backward_weight(

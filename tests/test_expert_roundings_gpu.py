@@ -76,3 +76,40 @@ def test_bias_gradient_sums_unrounded_values(counts, n):
     db, = torch.autograd.grad(y, b, torch.full_like(y, 129 / 128))
     expected = torch.tensor(counts, device='cuda')[:, None] * (387 / 512)
     assert db.dtype is torch.float32 and torch.equal(db, expected.expand(-1, n))
+
+
+@pytest.mark.parametrize('act', ['gelu', 'leaky_relu_0.01'])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16, torch.float32], ids=str)
+@pytest.mark.parametrize('rows,n', [(70, 40), (1400, 1032)])
+@pytest.mark.parametrize('eight', [False, True])
+def test_pre_activation_is_kept_where_the_caller_asks(act, dtype, rows, n, eight):
+    """
+    ``set_save_derivative(False)``: Z is kept in the layer's type instead of act'(Z), as in ``Linear``.  Whole numbers, exact
+    in every type, so that dZ is off by its own rounding and the evaluation of act' (a few 1e-6), and dW by those times the
+    rows (x is 0 or +-1) and its own rounding.
+    """
+    g = torch.Generator(device='cuda').manual_seed(rows)
+    x = torch.randint(-1, 2, (rows, 8), generator=g, device='cuda').to(dtype)
+    w = torch.randint(-1, 2, (2, 8, n), generator=g, device='cuda').to(dtype)
+    dy = torch.randn(rows, n, generator=g, device='cuda').to(dtype)
+    counts = [rows] if eight else [rows // 3, rows - rows // 3]
+    leaf = (w[0] if eight else w).clone().requires_grad_()
+    previous = attorch.set_save_derivative(False)
+    try:
+        y = attorch.Float8LinearAutoGrad.apply(x, leaf, None, act) if eight else \
+            attorch.grouped_linear(x, offsets_of(counts), leaf, None, act)
+    finally:
+        attorch.set_save_derivative(previous)
+    stack = leaf.detach().double().view(len(counts), 8, n)
+    groups = [(e, r) for e, r in enumerate(torch.arange(rows, device='cuda').split(counts))]
+    z64 = torch.cat([x[r].double() @ stack[e] for e, r in groups])
+    kept = y.grad_fn.saved_tensors[3]
+    assert kept.dtype is dtype and torch.equal(kept.double(), z64)
+    dw, = torch.autograd.grad(y, leaf, dy)
+    # fp32 operands are multiplied as TF32, which keeps 10 bits (a whole step of 2^-10 where they are cut off).
+    eps = 2.0 ** -10 if dtype is torch.float32 else torch.finfo(dtype).eps / 2
+    dz = dy.double() * act64(z64, act)[1]
+    size = dz.abs() * eps + dy.double().abs() * 4e-6 + 2.0 ** -25
+    expected = torch.stack([x[r].double().T @ dz[r] for _, r in groups]).view_as(leaf)
+    bound = torch.stack([x[r].double().abs().T @ (size[r] + rows * 2.0 ** -23 * dz[r].abs()) for _, r in groups]).view_as(leaf)
+    assert ((dw.double() - expected).abs() <= bound + eps * (expected.abs() + bound)).all()
