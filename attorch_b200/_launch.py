@@ -7,7 +7,7 @@ import contextlib
 
 import torch
 
-from .linear_layer import _scratch, _stream_scratch
+from .linear_layer import _status_words
 
 _CURRENT = contextlib.nullcontext()
 
@@ -22,16 +22,22 @@ def stream_of(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-def status_of(device: torch.device, stream: int) -> int:
-    """Address of the status word of a stream of ``device``, which is current (see ``check_status``)."""
-    entry = _scratch.get((device.index, stream))
-    if entry is None:
-        if torch.cuda.is_current_stream_capturing():
-            # Made inside the capture the word would be zeroed by the graph's replays only, and ``check_status`` before the
-            # first of them would read whatever is there.  Any other stream's word of the device serves: it is written
-            # by a wait that ran out and by nothing else.
-            for (index, _), other in _scratch.items():
-                if index == device.index:
-                    return other['status'].data_ptr()
-        entry = _stream_scratch(device)
-    return entry['status'].data_ptr()
+def status_of(device: torch.device) -> int:
+    """
+    Address of the device's status word (see ``check_status``).  All streams share it: it is written by a wait that ran out
+    and by nothing else.  It is never dropped, because captured graphs hold its address.
+    """
+    word = _status_words.get(device.index)
+    return (_new_status_word(device) if word is None else word).data_ptr()
+
+
+def _new_status_word(device: torch.device) -> torch.Tensor:
+    word = torch.empty(1, dtype=torch.int32, device=device)
+    if torch.cuda.is_current_stream_capturing():
+        # Recorded in the capture, the zeroing would only run with the graph's replays, and ``check_status`` before the first
+        # of them would read whatever is there.  It runs now, on a stream that is not captured.
+        with torch.cuda.stream(torch.cuda.Stream(device)):
+            word.zero_()
+    else:
+        word.zero_()
+    return _status_words.setdefault(device.index, word)          # another thread may have been first

@@ -275,7 +275,7 @@ class GateAutoGrad(torch.autograd.Function):
             output = torch.empty((rows, experts), dtype=dtype, device=input.device)
             _lib.check(lib.ab200_grouped_linear_forward(
                 _ptr(x_op), _ptr(w_op), None, None, None, _ptr(output), rows, 1, in_dim, experts, _pitch(x_op), 0, _pitch(w_op),
-                experts, experts, _dtype_id(dtype), 0, _lib.ACT_NONE, 0.0, status_of(input.device, stream), stream,
+                experts, experts, _dtype_id(dtype), 0, _lib.ACT_NONE, 0.0, status_of(input.device), stream,
                 _flags_for(input.device)), 'ab200_grouped_linear_forward')
         ctx.dtypes = (input.dtype, weight.dtype)
         ctx.needs = (input.requires_grad, weight.requires_grad)
@@ -291,7 +291,7 @@ class GateAutoGrad(torch.autograd.Function):
         input_grad = weight_grad = None
         with on(device):
             stream = stream_of(device)
-            status = status_of(device, stream)
+            status = status_of(device)
             dy = _rows_operand(output_grad, dtype, stream)
             dt = _dtype_id(dtype)
 

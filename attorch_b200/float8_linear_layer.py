@@ -111,7 +111,7 @@ def _product(xq: Tensor, x_scale: Tensor, wq: Tensor, w_scale: Tensor, scale_str
         _ptr(xq), _ptr(x_scale), _ptr(wq), _ptr(w_scale), _ptr(bias), _ptr(offsets), _ptr(pre_act), _ptr(out), rows,
         wq.shape[0] if grouped else 1, k, n, _padded(k), x_scale.shape[1], wq.stride(0) if grouped and wq.shape[0] > 1 else n * pitch,
         pitch, *scale_strides, n, n, _dtype_id(out.dtype), _dtype_id(bias.dtype) if bias is not None else 0, act, param,
-        status_of(device, stream), stream, _flags_for(device) | extra_flags), 'ab200_float8_product')
+        status_of(device), stream, _flags_for(device) | extra_flags), 'ab200_float8_product')
 
 
 def _check_stored(input: Tensor, weight: Tensor, scale: Tensor, bias: Optional[Tensor], ndim: int) -> None:
@@ -235,7 +235,7 @@ class Float8LinearAutoGrad(torch.autograd.Function):
         input_grad = weight_grad = bias_grad = None
         with on(device):
             stream = stream_of(device)
-            status = status_of(device, stream)
+            status = status_of(device)
             dt = _dtype_id(dtype)
             dy = _rows_operand(output_grad.reshape(rows, out_dim), dtype, stream)
             dz = dy

@@ -123,7 +123,7 @@ def _forward(input: Tensor, offsets: Tensor, weight: Tensor, bias: Optional[Tens
     lib = _lib.load()
     with on(input.device):
         stream = stream_of(input.device)
-        status = status_of(input.device, stream)
+        status = status_of(input.device)
         x_op = _rows_operand(input, out_dtype, stream)
         w_op = _stack_operand(weight, out_dtype, stream)
         bias_op = bias if bias is None or bias.is_contiguous() else bias.contiguous()
@@ -159,7 +159,7 @@ class GroupedLinearAutoGrad(torch.autograd.Function):
         input_grad = weight_grad = bias_grad = None
         with on(device):
             stream = stream_of(device)
-            status = status_of(device, stream)
+            status = status_of(device)
             flags = _flags_for(device)
             dy = _rows_operand(output_grad, dtype, stream)
             dz = dy

@@ -23,6 +23,8 @@ _DTYPE_IDS = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: 
 # Per (device index, stream) scratch: a grow-only workspace and the device status word.
 _scratch: Dict[Tuple[int, int], Dict[str, Tensor]] = {}
 _scratch_clock = 0
+# Per device index: the status word of the calls that keep no scratch (see _launch.status_of).
+_status_words: Dict[int, Tensor] = {}
 
 # Flags forwarded to every GEMM entry point (tests use them to pin a kernel family).
 _gemm_flags = 0
@@ -137,12 +139,15 @@ def check_status(device: Optional[torch.device] = None) -> None:
     own; call this where the program synchronises anyway.
     """
     failure = None
-    for key, entry in list(_scratch.items()):
-        if device is not None and device.index is not None and device.index != key[0]:
-            continue
-        code = int(entry['status'].item())          # synchronises with the stream that last used the entry
+    words = [(key[0], entry['status']) for key, entry in list(_scratch.items())] + list(_status_words.items())
+    if device is not None and device.index is not None:
+        words = [(index, word) for index, word in words if index == device.index]
+    for index in {index for index, _ in words}:
+        torch.cuda.synchronize(index)               # a word is written by kernels of any stream
+    for _, word in words:
+        code = int(word.item())
         if code != 0 and failure is None:
-            entry['status'].zero_()
+            word.zero_()
             failure = code
     _trim_scratch()
     if failure is not None:

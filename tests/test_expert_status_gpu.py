@@ -1,0 +1,67 @@
+"""The status word of the experts' and 8-bit products: one a device, held for good, read by check_status."""
+
+import pytest
+import torch
+
+import attorch_b200 as attorch
+from attorch_b200 import _lib, linear_layer
+from attorch_b200._launch import status_of
+
+pytestmark = pytest.mark.gpu
+
+
+def captured_call():
+    """A graph of one grouped product, captured on a stream of its own, and the address its kernel reports to."""
+    x, w = torch.ones(20, 32, device='cuda'), torch.ones(2, 32, 48, device='cuda')
+    offsets = torch.tensor([0, 7, 20], dtype=torch.int32, device='cuda')
+    attorch.grouped_linear(x, offsets, w)                     # loads the kernels outside the capture
+    torch.cuda.synchronize()
+    return x, w, offsets
+
+
+def test_word_outlives_idle_streams_and_is_read():
+    """A graph keeps the address after its stream has long been idle; what a replay stores there is reported."""
+    x, w, offsets = captured_call()
+    device = x.device
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        y = attorch.grouped_linear(x, offsets, w)
+        address = status_of(device)
+    layer = attorch.Linear(64, 64)
+    rows = torch.randn(32, 64, device='cuda')
+    for stream in [torch.cuda.Stream() for _ in range(linear_layer._MAX_SCRATCH_ENTRIES + 8)]:
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            layer(rows)
+    attorch.check_status()                                    # drops the scratch of idle streams
+    word = linear_layer._status_words[device.index]
+    assert word.data_ptr() == address == status_of(device)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, torch.full_like(y, 32.0))
+    word.fill_(2)                                             # what a wait that ran out stores
+    with pytest.raises(_lib.LibraryError, match='device status 2'):
+        attorch.check_status(device)
+    attorch.check_status()
+
+
+def test_word_made_inside_a_capture_is_valid_at_once():
+    """No call before the capture had made a word: it is zero before the graph has run, and replays leave it alone."""
+    x, w, offsets = captured_call()
+    index = x.device.index
+    held = linear_layer._status_words.pop(index)
+    filler = torch.full((1 << 20,), -1, dtype=torch.int32, device='cuda')
+    del filler                                                # memory handed out next is not zero
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+            y = attorch.grouped_linear(x, offsets, w)
+        attorch.check_status()
+        linear_layer._status_words[index].fill_(3)
+        graph.replay()
+        with pytest.raises(_lib.LibraryError, match='device status 3'):
+            attorch.check_status()
+        attorch.check_status()
+        assert torch.equal(y, torch.full_like(y, 32.0))
+    finally:
+        linear_layer._status_words[index] = held
