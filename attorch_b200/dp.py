@@ -102,7 +102,7 @@ class GradientBuckets:
     destinations, its parameters' ``.grad`` alias it, and a callback all-reduces the layer's slice.
 
     Args:
-        layers: The Linear layers, in forward order.
+        layers: The Linear layers, in forward order (a Router's ``gate`` is one); others are refused.
         process_group: Group to reduce over; None for the default group.  With a world size of 1
             (or torch.distributed not initialised) no collective is issued.
         overlap: Issue each layer's all-reduce on a side stream as soon as its gradients are
@@ -131,6 +131,10 @@ class GradientBuckets:
                  grad_dtype: Optional[torch.dtype] = None, exchange: bool = True, transport: str = 'nccl',
                  comm_ctas: int = 8) -> None:
         self.layers: List[Linear] = list(layers)
+        for layer in self.layers:
+            # The other layers return their gradients to autograd, which would add them to a view of the bucket.
+            if not hasattr(layer, 'weight_grad_out') or not getattr(layer, 'writes_into_buckets', True):
+                raise TypeError(f'{type(layer).__name__} does not write its gradients into a bucket: reduce its .grad after backward')
         self.group = process_group
         self.world_size = dist.get_world_size(process_group) if (dist.is_initialized() and exchange) else 1
         first = self.layers[0].weight

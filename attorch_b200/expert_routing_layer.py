@@ -255,10 +255,12 @@ class GateAutoGrad(torch.autograd.Function):
     ``apply(input, weight)``: ``input @ weight`` with the bits of a row independent of timing.  ``Linear`` shares the
     reduction of a product this narrow out over all SMs and adds the pieces atomically, in an order that changes
     from call to call; a token whose logits nearly tie could then change its experts.  The grouped kernel with one
-    group sums every output in one place.  Backward is ``Linear``'s.
+    group sums every output in one place.  Backward is ``Linear``'s, and the optional trailing arguments are those of
+    ``LinearAutoGrad`` for data-parallel training (where ``dW`` goes, who is told, what is put off).
     """
     @staticmethod
-    def forward(ctx, input: Tensor, weight: Tensor) -> Tensor:
+    def forward(ctx, input: Tensor, weight: Tensor, weight_grad_out: Optional[Tensor] = None, grad_ready=None,
+                dw_chunks: int = 1, defer_input_grad=None) -> Tensor:
         assert input.ndim == 2 and input.shape[1] == weight.shape[0], \
             f'Incompatible input ({input.shape}) and weights ({weight.shape}) shape'
         assert weight.device == input.device, f'The weights are on {weight.device}, the input on {input.device}'
@@ -279,6 +281,8 @@ class GateAutoGrad(torch.autograd.Function):
                 _flags_for(input.device)), 'ab200_grouped_linear_forward')
         ctx.dtypes = (input.dtype, weight.dtype)
         ctx.needs = (input.requires_grad, weight.requires_grad)
+        ctx.weight_grad_out, ctx.grad_ready, ctx.dw_chunks = weight_grad_out, grad_ready, int(dw_chunks)
+        ctx.defer_input_grad = defer_input_grad
         ctx.save_for_backward(x_op, w_op)
         return output
 
@@ -287,33 +291,59 @@ class GateAutoGrad(torch.autograd.Function):
         x_op, w_op = ctx.saved_tensors
         rows, in_dim = x_op.shape
         experts, dtype, device = w_op.shape[1], x_op.dtype, x_op.device
-        lib = _lib.load()
+        dt = _dtype_id(dtype)
         input_grad = weight_grad = None
         with on(device):
-            stream = stream_of(device)
-            status = status_of(device)
-            dy = _rows_operand(output_grad, dtype, stream)
-            dt = _dtype_id(dtype)
-
-            def scratch(*shape: int) -> Tuple[Optional[Tensor], int]:
-                nbytes = _cached_size('ab200_gemm_workspace_bytes', *shape)
-                return (torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None), nbytes
-
+            dy = _rows_operand(output_grad, dtype, stream_of(device))
             if ctx.needs[1]:
-                weight_grad = torch.empty((in_dim, experts), dtype=ctx.dtypes[1], device=device)
-                workspace, nbytes = scratch(in_dim, experts, rows)
-                _lib.check(lib.ab200_linear_backward_weight(
-                    _ptr(x_op), _ptr(dy), _ptr(weight_grad), rows, in_dim, experts, _pitch(x_op), 1, _pitch(dy), 1, experts, dt,
-                    _dtype_id(weight_grad.dtype), _ptr(workspace), nbytes, status, stream, _flags_for(device)),
-                    'ab200_linear_backward_weight')
+                weight_grad = ctx.weight_grad_out if ctx.weight_grad_out is not None else \
+                    torch.empty((in_dim, experts), dtype=ctx.dtypes[1], device=device)
+                # Blocks of rows of dW, each handed to the gradient exchange as soon as it is enqueued.
+                blocks = ctx.dw_chunks if ctx.grad_ready is not None and ctx.dw_chunks > 1 and in_dim % (ctx.dw_chunks * 8) == 0 else 1
+                size = in_dim // blocks
+                for block in range(blocks):
+                    _gate_weight_grad(x_op[:, block * size:(block + 1) * size], dy, weight_grad[block * size:(block + 1) * size])
+                    if ctx.grad_ready is not None:
+                        ctx.grad_ready(block, blocks)
+            elif ctx.grad_ready is not None:
+                ctx.grad_ready(0, 1)
             if ctx.needs[0]:
                 input_grad = torch.empty((rows, in_dim), dtype=ctx.dtypes[0], device=device)
-                workspace, nbytes = scratch(rows, in_dim, experts)
-                _lib.check(lib.ab200_linear_backward_input(
-                    _ptr(dy), _ptr(w_op), _ptr(input_grad), rows, in_dim, experts, _pitch(dy), 1, _pitch(w_op), 1, in_dim, dt,
-                    _dtype_id(input_grad.dtype), _ptr(workspace), nbytes, status, stream, _flags_for(device)),
-                    'ab200_linear_backward_input')
-        return input_grad, weight_grad
+                address, row_bytes, dx_dtype = input_grad.data_ptr(), in_dim * input_grad.element_size(), _dtype_id(input_grad.dtype)
+
+                # Holds dY and W alive but not dX, which autograd is to be the only owner of (see LinearAutoGrad).
+                def launch_input_grad(row_begin=0, row_end=None, dz=dy, w=w_op):
+                    count = min(rows, rows if row_end is None else row_end) - row_begin
+                    if count <= 0:
+                        return
+                    with on(device):
+                        workspace, nbytes = _gemm_workspace(device, count, in_dim, experts)
+                        _lib.check(_lib.load().ab200_linear_backward_input(
+                            dz.data_ptr() + row_begin * _pitch(dz) * dz.element_size(), _ptr(w), address + row_begin * row_bytes,
+                            count, in_dim, experts, _pitch(dz), 1, _pitch(w), 1, in_dim, dt, dx_dtype, _ptr(workspace), nbytes,
+                            status_of(device), stream_of(device), _flags_for(device)), 'ab200_linear_backward_input')
+
+                if ctx.defer_input_grad is not None:
+                    ctx.defer_input_grad(launch_input_grad)
+                else:
+                    launch_input_grad()
+        # A gradient that went to the caller's buffer is not returned as well: autograd would add it to ``.grad``.
+        return input_grad, None if ctx.weight_grad_out is not None else weight_grad, None, None, None, None
+
+
+def _gemm_workspace(device: torch.device, *shape: int) -> Tuple[Optional[Tensor], int]:
+    nbytes = _cached_size('ab200_gemm_workspace_bytes', *shape)
+    return (torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None), nbytes
+
+
+def _gate_weight_grad(x: Tensor, dy: Tensor, out: Tensor) -> None:
+    """out = x^T dy."""
+    (rows, in_dim), experts = x.shape, dy.shape[1]
+    workspace, nbytes = _gemm_workspace(x.device, in_dim, experts, rows)
+    _lib.check(_lib.load().ab200_linear_backward_weight(
+        _ptr(x), _ptr(dy), _ptr(out), rows, in_dim, experts, _pitch(x), 1, _pitch(dy), 1, experts, _dtype_id(x.dtype),
+        _dtype_id(out.dtype), _ptr(workspace), nbytes, status_of(x.device), stream_of(x.device), _flags_for(x.device)),
+        'ab200_linear_backward_weight')
 
 
 class Router(nn.Module):
@@ -342,4 +372,6 @@ class Router(nn.Module):
 
     def forward(self, input: Tensor, mask: Optional[Tensor] = None) -> Routing:
         """``input``: ``[tokens, dim]``; ``mask``: see ``route``."""
-        return route(GateAutoGrad.apply(input, self.gate.weight), self.top_k, self.score_func, self.renormalize, mask)
+        gate = self.gate
+        logits = GateAutoGrad.apply(input, gate.weight, gate.weight_grad_out, gate.grad_ready, gate.dw_chunks, gate.defer_input_grad)
+        return route(logits, self.top_k, self.score_func, self.renormalize, mask)

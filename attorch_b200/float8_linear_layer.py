@@ -285,6 +285,8 @@ class Float8Linear(Linear):
         device: Device to use.
         dtype: Dtype of the parameters.
     """
+    writes_into_buckets = False         # see dp.GradientBuckets
+
     def __init__(self, in_features: int, out_features: int, bias: bool = True, act_func: Optional[str] = None,
                  device='cuda', dtype: torch.dtype = torch.float32) -> None:
         super().__init__(in_features, out_features, bias, act_func, device, dtype)

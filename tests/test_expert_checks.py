@@ -24,3 +24,17 @@ def test_gate_refuses_weights_of_another_device():
     router = attorch.Router(8, 4, 2, device='meta')
     with pytest.raises(AssertionError, match='weights are on meta'):
         router(torch.zeros(3, 8))
+
+
+def test_buckets_refuse_layers_that_do_not_write_into_them():
+    """Their .grad would be a view of a bucket that nothing of theirs is written to, exchanged or cleared in."""
+    from attorch_b200.dp import GradientBuckets
+    linear = attorch.Linear(4, 6, device='cpu')
+    with pytest.raises(TypeError, match='GroupedLinear'):
+        GradientBuckets([linear, attorch.GroupedLinear(2, 4, 6, device='cpu')])
+    with pytest.raises(TypeError, match='Float8Linear'):
+        GradientBuckets([attorch.Float8Linear(4, 6, device='cpu')])
+    assert linear.weight_grad_out is None and linear.weight.grad is None       # refused before anything was changed
+    gate = attorch.Router(4, 6, 2, device='cpu').gate
+    buckets = GradientBuckets([linear, gate])
+    assert gate.weight.grad.data_ptr() == gate.weight_grad_out.data_ptr() == buckets.flat[30:].data_ptr()
