@@ -4,8 +4,10 @@ public forms of these three took 6 of the 28 microseconds of a one-token call.
 """
 
 import contextlib
+from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from .linear_layer import _status_words
 
@@ -20,6 +22,22 @@ def on(device: torch.device):
 def stream_of(device: torch.device) -> int:
     """The current stream of ``device`` as an address."""
     return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def recorded(*tensors: Optional[torch.Tensor]) -> bool:
+    """
+    Whether a call goes through its autograd function: something asks for a gradient, or an input may carry a forward-mode
+    tangent, which PyTorch then refuses (there are no such derivatives) where the bare call would drop it.
+    """
+    if forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any(tensor is not None and tensor.requires_grad for tensor in tensors)
+
+
+def has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether one of the tensors carries a forward-mode tangent."""
+    return forward_ad._current_level >= 0 and \
+        any(tensor is not None and forward_ad.unpack_dual(tensor).tangent is not None for tensor in tensors)
 
 
 def status_of(device: torch.device) -> int:

@@ -14,7 +14,7 @@ import torch
 from torch import Tensor, nn
 
 from . import _lib
-from ._launch import on, status_of, stream_of
+from ._launch import on, recorded, status_of, stream_of
 from .grouped_linear_layer import _pitch, _rows_operand
 from .linear_layer import (Linear, _cached_size, _dtype_id, _flags_for, _ptr, _require_cuda,
                            get_output_dtype)
@@ -129,7 +129,7 @@ def route(logits: Tensor, top_k: int, score_func: str = 'softmax', renormalize: 
         renormalize: Flag for dividing a token's weights by their sum.
         mask: Optional ``[tokens]`` boolean; False (padding) sends a token to no expert.
     """
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if recorded(logits):
         return Routing(*RouteAutoGrad.apply(logits, top_k, score_func, renormalize, mask))
     return Routing(*_route(logits, top_k, score_func, renormalize, mask, False)[0])
 
@@ -224,7 +224,7 @@ def dispatch(input: Tensor, routing: Routing) -> Tensor:
     _require_cuda(input, 'input')
     _dtype_id(input.dtype)
     _check_plan(routing, input.device, input.shape[0])
-    if torch.is_grad_enabled() and input.requires_grad:
+    if recorded(input):
         return DispatchAutoGrad.apply(input, routing.token_row, routing.offsets)
     return _dispatch(input, routing.token_row, routing.offsets)
 
@@ -245,7 +245,7 @@ def combine(rows: Tensor, routing: Routing) -> Tensor:
         'weights must be fp32, one per choice, on the device of the rows'
     if not weights.is_contiguous():
         weights = weights.contiguous()
-    if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
+    if recorded(rows, weights):
         return CombineAutoGrad.apply(rows, weights, routing.token_row, routing.offsets)
     return _combine(rows, routing.token_row, weights)
 

@@ -19,7 +19,7 @@ import torch
 from torch import Tensor, nn
 
 from . import _lib
-from ._launch import on, status_of, stream_of
+from ._launch import has_tangent, on, status_of, stream_of
 from .acts import act_id, parse_act_func
 from .grouped_linear_layer import MAX_GROUPS, GroupedLinear, _check_offsets, _kept_for_backward, _pitch, _rows_operand
 from .linear_layer import Linear, _cached_size, _dtype_id, _flags_for, _ptr, _require_cuda, get_output_dtype
@@ -130,6 +130,8 @@ def _check_stored(input: Tensor, weight: Tensor, scale: Tensor, bias: Optional[T
     if torch.is_grad_enabled() and (input.requires_grad or (bias is not None and bias.requires_grad)):
         raise RuntimeError('Products with stored 8-bit weights have no gradient: train with Float8Linear, or call them under '
                            'torch.no_grad().')
+    if has_tangent(input, scale, bias):
+        raise NotImplementedError('Products with stored 8-bit weights have no forward-mode derivative.')
 
 
 def _stored(input: Tensor, offsets: Optional[Tensor], weight: Tensor, scale: Tensor, bias: Optional[Tensor],

@@ -18,7 +18,7 @@ from torch import Tensor, nn
 
 from . import _lib
 from . import linear_layer as _layer
-from ._launch import on, status_of, stream_of
+from ._launch import on, recorded, status_of, stream_of
 from .acts import act_id, parse_act_func
 from .linear_layer import _cached_size, _dtype_id, _flags_for, _ptr, _require_cuda, get_output_dtype
 
@@ -205,7 +205,7 @@ def grouped_linear(input: Tensor, offsets: Tensor, weight: Tensor, bias: Optiona
         bias: ``[groups, out_features]`` or None.
         act_func: Activation, as ``Linear``.
     """
-    if torch.is_grad_enabled() and (input.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+    if recorded(input, weight, bias):
         return GroupedLinearAutoGrad.apply(input, offsets, weight, bias, act_func)
     return _forward(input, offsets, weight, bias, act_func, False)[0]
 
