@@ -303,13 +303,17 @@ class Float8Linear(Linear):
         return layer
 
     def freeze(self) -> 'Float8Linear':
-        """Replaces the weight by its 8-bit form (half of bf16's memory) and the bias by a constant; returns the layer."""
+        """
+        Replaces the weight by its 8-bit form (half of bf16's memory) and the bias by a constant copy; returns the layer.  A
+        layer that shares the parameters keeps them as they are.
+        """
         if self.weight is None:
             return self
         self.weight_float8, self.weight_scale = quantize_weight(self.weight)
         self.weight = None
         if self.bias is not None:
-            self.bias.requires_grad_(False)
+            # A snapshot like the weight's: the parameter may be another layer's too (from_linear), which goes on training it.
+            self.bias = nn.Parameter(self.bias.detach().clone(), requires_grad=False)
         return self
 
     def forward(self, input: Tensor, residual: Optional[Tensor] = None) -> Tensor:
@@ -345,7 +349,7 @@ class Float8GroupedLinear(nn.Module):
     def from_grouped(cls, grouped: GroupedLinear) -> 'Float8GroupedLinear':
         """The 8-bit form of a ``GroupedLinear``."""
         weight, scale = quantize_weight(grouped.weight)
-        return cls(weight, scale, grouped.bias, grouped.act_func)
+        return cls(weight, scale, None if grouped.bias is None else grouped.bias.detach().clone(), grouped.act_func)
 
     def forward(self, input: Tensor, offsets: Tensor) -> Tensor:
         return float8_grouped_linear(input, offsets, self.weight, self.scale, self.bias, self.act_func)

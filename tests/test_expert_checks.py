@@ -38,3 +38,24 @@ def test_buckets_refuse_layers_that_do_not_write_into_them():
     gate = attorch.Router(4, 6, 2, device='cpu').gate
     buckets = GradientBuckets([linear, gate])
     assert gate.weight.grad.data_ptr() == gate.weight_grad_out.data_ptr() == buckets.flat[30:].data_ptr()
+
+
+def test_frozen_copies_leave_the_trained_layer_alone(monkeypatch):
+    """The 8-bit form of a layer in training is a snapshot: the layer's parameters still train, and do not reach the copy."""
+    from attorch_b200 import float8_linear_layer
+
+    def snapshot(weight):
+        return weight.detach().transpose(-1, -2).contiguous().to(torch.float8_e4m3fn), torch.ones(*weight.shape[:-2], 1, 1)
+
+    monkeypatch.setattr(float8_linear_layer, 'quantize_weight', snapshot)
+    linear = attorch.Linear(16, 32, device='cpu')
+    frozen = attorch.Float8Linear.from_linear(linear).freeze()
+    grouped = attorch.GroupedLinear(2, 16, 32, device='cpu')
+    eight = attorch.Float8GroupedLinear.from_grouped(grouped)
+    for source, copy in ((linear, frozen), (grouped, eight)):
+        assert source.weight.requires_grad and source.bias.requires_grad and not copy.bias.requires_grad
+        before = copy.bias.clone()
+        assert torch.equal(before, source.bias)
+        with torch.no_grad():
+            source.bias.add_(1.0)
+        assert torch.equal(copy.bias, before)
