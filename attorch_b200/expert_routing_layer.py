@@ -71,20 +71,20 @@ def _route(logits: Tensor, top_k: int, score_func: str, renormalize: bool, mask:
     with on(device):
         stream = stream_of(device)
         weights = torch.empty((tokens, top_k), dtype=torch.float32, device=device)
-        # Whole numbers share one allocation; the C entry takes their addresses.
-        slots = tokens * top_k
-        plan = torch.empty(3 * slots + experts + 1, dtype=torch.int32, device=device)
-        chosen, token_row, row_token, offsets = plan.split((slots, slots, slots, experts + 1))
+        # Tensors of their own, not parts of one: parts share a version counter, and a caller who edits the plan in place would
+        # then seem to have changed `chosen`, which backward reads.
+        chosen = torch.empty((tokens, top_k), dtype=torch.int32, device=device)
+        token_row = torch.empty((tokens, top_k), dtype=torch.int32, device=device)
+        row_token = torch.empty(tokens * top_k, dtype=torch.int32, device=device)
+        offsets = torch.empty(experts + 1, dtype=torch.int32, device=device)
         stats = torch.empty((tokens, 2), dtype=torch.float32, device=device) if needs_grad else None
         ws_bytes = _cached_size('ab200_route_workspace_bytes', tokens, experts)
         workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
-        at = plan.data_ptr()
         _lib.check(lib.ab200_route_forward(
-            _ptr(logits), _ptr(mask), _ptr(weights), at, _ptr(stats), at + 12 * slots, at + 8 * slots, at + 4 * slots, tokens,
-            experts, top_k, _pitch(logits), dtype, _SCORE_FUNCS[score_func], int(bool(renormalize)), _ptr(workspace), ws_bytes,
-            stream), 'ab200_route_forward')
-    routing = (weights, chosen.view(tokens, top_k), offsets, row_token, token_row.view(tokens, top_k))
-    return routing, logits, stats
+            _ptr(logits), _ptr(mask), _ptr(weights), _ptr(chosen), _ptr(stats), _ptr(offsets), _ptr(row_token), _ptr(token_row),
+            tokens, experts, top_k, _pitch(logits), dtype, _SCORE_FUNCS[score_func], int(bool(renormalize)), _ptr(workspace),
+            ws_bytes, stream), 'ab200_route_forward')
+    return (weights, chosen, offsets, row_token, token_row), logits, stats
 
 
 class RouteAutoGrad(torch.autograd.Function):
