@@ -422,10 +422,12 @@ int ab200_expert_dispatch(const void* x, const int* token_row, const int* row_en
   const int per = vec ? 16 / elt : 1;
   const int64_t units = dim / per;
   const dim3 block = row_block(units);
-  const unsigned grid = row_grid(tokens > 0 ? tokens : rows, block, 16);
+  const int clearing = clear_blocks(rows);
+  const unsigned grid = row_grid(tokens > 0 ? tokens : rows, block, 16) + clearing;
 #define AB200_DISPATCH(V)                                                                                                  \
-  dispatch_kernel<V><<<grid, block, 0, stream>>>(static_cast<const V*>(x), ld_x / per, token_row, row_end,                 \
-      static_cast<V*>(rows_out), units, static_cast<int>(tokens), static_cast<int>(top_k), static_cast<int>(rows), static_cast<int>(units))
+  dispatch_kernel<V><<<grid, block, clear_smem_bytes(rows), stream>>>(static_cast<const V*>(x), ld_x / per, token_row,     \
+      row_end, static_cast<V*>(rows_out), units, static_cast<int>(tokens), static_cast<int>(top_k), static_cast<int>(rows), \
+      static_cast<int>(units), clearing)
   if (vec) AB200_DISPATCH(uint4);
   else if (elt == 4) AB200_DISPATCH(uint32_t);
   else AB200_DISPATCH(uint16_t);
@@ -483,11 +485,13 @@ int ab200_expert_combine_backward(const void* dy, const void* rows_in, const int
   const int per = vec ? 16 / elt : 1;
   const int64_t units = dim / per;
   const dim3 block = row_block(units);
-  const unsigned grid = row_grid(tokens > 0 ? tokens : rows, block, 16);
+  const int clearing = rows_grad ? clear_blocks(rows) : 0;
+  const unsigned grid = row_grid(tokens > 0 ? tokens : rows, block, 16) + clearing;
+  const int smem = rows_grad && rows > 0 ? clear_smem_bytes(rows) : 0;
 #define AB200_COMBINE_BWD(T, V)                                                                                             \
-  combine_backward_kernel<T, V><<<grid, block, 0, stream>>>(static_cast<const T*>(dy), ld_dy, static_cast<const T*>(rows_in), \
+  combine_backward_kernel<T, V><<<grid, block, smem, stream>>>(static_cast<const T*>(dy), ld_dy, static_cast<const T*>(rows_in), \
       ld_rows, token_row, weights, row_end, static_cast<T*>(rows_grad), weights_grad, static_cast<int>(tokens),             \
-      static_cast<int>(top_k), static_cast<int>(rows), static_cast<int>(units), static_cast<int>(dim))
+      static_cast<int>(top_k), static_cast<int>(rows), static_cast<int>(units), static_cast<int>(dim), clearing)
   if (dtype == DT_F32) { if (vec) AB200_COMBINE_BWD(float, 4); else AB200_COMBINE_BWD(float, 1); }
   else if (dtype == DT_F16) { if (vec) AB200_COMBINE_BWD(__half, 8); else AB200_COMBINE_BWD(__half, 1); }
   else { if (vec) AB200_COMBINE_BWD(__nv_bfloat16, 8); else AB200_COMBINE_BWD(__nv_bfloat16, 1); }

@@ -365,23 +365,68 @@ route_backward_kernel(const T* __restrict__ logits, long long ld, const float* _
 // its k copies, the sums read k rows and write one; no row list is needed and nothing is added atomically.
 // ------------------------------------------------------------------------------------------------
 
-// rows[token_row[t, j]] = x[t], and zeros in the rows behind the last group.  V: 16-, 4- or 2-byte units.
+// Rows below `end` that no entry of token_row names (choices that the caller has dropped) become zeros.  The first
+// gridDim.x - work blocks of a kernel each take a run of num_rows / blocks rows: all entries are read (a few tens of blocks
+// read 4 bytes a row each, from L2), those that fall into the run are marked in shared memory, and what is left is
+// cleared.  It runs beside the moves of the other blocks, which write the rows that are named and those from `end` on.
+constexpr int kClearBlocks = 32, kClearRows = 1 << 18;       // blocks at most, unless a run would pass kClearRows
+inline int clear_blocks(long long rows) {
+  const long long least = (rows + kClearRows - 1) / kClearRows, want = (rows + 1023) / 1024;
+  return static_cast<int>(want < kClearBlocks ? want : (least > kClearBlocks ? least : kClearBlocks));
+}
+inline int clear_smem_bytes(long long rows) {
+  const long long run = (rows + clear_blocks(rows) - 1) / clear_blocks(rows);
+  return static_cast<int>((run + 31) / 32 * 4);
+}
+template <class V>
+__device__ __forceinline__ void clear_unnamed(V* __restrict__ rows, long long ld_rows, int units, const int* __restrict__ token_row,
+                                              long long entries, int num_rows, int end, int blocks, uint32_t* named) {
+  const int thread = threadIdx.y * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y;
+  const int lane = thread & 31;
+  const long long run = (static_cast<long long>(num_rows) + blocks - 1) / blocks;
+  const long long begin = blockIdx.x * run;
+  const int count = static_cast<int>(min(run, max(end - begin, 0ll)));
+  for (int i = thread; i < (count + 31) / 32; i += threads) named[i] = 0u;
+  __syncthreads();
+#pragma unroll 8
+  for (long long i = thread; i < entries; i += threads) {
+    const long long r = __ldg(token_row + i) - begin;
+    if (r >= 0 && r < count) atomicOr(&named[r >> 5], 1u << (r & 31));
+  }
+  __syncthreads();
+  for (int w = thread >> 5; w < (count + 31) / 32; w += threads >> 5) {
+    uint32_t missing = ~named[w];
+    if (count - w * 32 < 32) missing &= (1u << (count - w * 32)) - 1u;
+    for (; missing != 0u; missing &= missing - 1u) {
+      const long long r = begin + w * 32 + __ffs(missing) - 1;
+      for (int u = lane; u < units; u += 32) rows[r * ld_rows + u] = V{};
+    }
+  }
+}
+
+// rows[token_row[t, j]] = x[t], and zeros in all other rows.  V: 16-, 4- or 2-byte units.
 template <class V>
 __global__ void __launch_bounds__(256)
 dispatch_kernel(const V* __restrict__ x, long long ld_x, const int* __restrict__ token_row, const int* __restrict__ row_end,
-                V* __restrict__ rows, long long ld_rows, int tokens, int k, int num_rows, int units) {
-  for (int t = blockIdx.x * blockDim.y + threadIdx.y; t < tokens; t += gridDim.x * blockDim.y) {
+                V* __restrict__ rows, long long ld_rows, int tokens, int k, int num_rows, int units, int clearing) {
+  extern __shared__ uint32_t named_rows[];
+  const int end = min(max(__ldg(row_end), 0), num_rows);
+  if (static_cast<int>(blockIdx.x) < clearing) {
+    clear_unnamed(rows, ld_rows, units, token_row, static_cast<long long>(tokens) * k, num_rows, end, clearing, named_rows);
+    return;
+  }
+  const int block = blockIdx.x - clearing, blocks = gridDim.x - clearing;
+  for (int t = block * blockDim.y + threadIdx.y; t < tokens; t += blocks * blockDim.y) {
     const int* at = token_row + static_cast<long long>(t) * k;
     for (int u = threadIdx.x; u < units; u += blockDim.x) {
       const V v = x[t * ld_x + u];
       for (int j = 0; j < k; ++j) {
         const int r = __ldg(at + j);
-        if (r >= 0 && r < num_rows) rows[r * ld_rows + u] = v;
+        if (r >= 0 && r < end) rows[r * ld_rows + u] = v;
       }
     }
   }
-  const int end = min(max(*row_end, 0), num_rows);
-  for (int r = end + blockIdx.x * blockDim.y + threadIdx.y; r < num_rows; r += gridDim.x * blockDim.y)
+  for (int r = end + block * blockDim.y + threadIdx.y; r < num_rows; r += blocks * blockDim.y)
     for (int u = threadIdx.x; u < units; u += blockDim.x) rows[r * ld_rows + u] = V{};
 }
 
@@ -438,18 +483,27 @@ combine_kernel(const T* __restrict__ rows, long long ld_rows, const int* __restr
   }
 }
 
-// drows[token_row[t, j]] = w[t, j] dy[t] (zeros behind the last group), dw[t, j] = <dy[t], rows[token_row[t, j]]>.
+// drows[token_row[t, j]] = w[t, j] dy[t] (zeros in all other rows), dw[t, j] = <dy[t], rows[token_row[t, j]]>.
 // Either output may be NULL.
 template <class T, int kVec>
 __global__ void __launch_bounds__(256)
 combine_backward_kernel(const T* __restrict__ dy, long long ld_dy, const T* __restrict__ rows, long long ld_rows,
                         const int* __restrict__ token_row, const float* __restrict__ weights, const int* __restrict__ row_end,
-                        T* __restrict__ drows, float* __restrict__ dweights, int tokens, int k, int num_rows, int units, int dim) {
+                        T* __restrict__ drows, float* __restrict__ dweights, int tokens, int k, int num_rows, int units, int dim,
+                        int clearing) {
   using U = RowUnit<T, kVec>;
+  extern __shared__ uint32_t named_rows[];
   __shared__ float part[8][kMaxTopK][8];                // [token of the block][j][warp of the token]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int warps = blockDim.x >> 5;
-  for (int tb = blockIdx.x * blockDim.y; tb < tokens; tb += gridDim.x * blockDim.y) {
+  const int end = min(max(__ldg(row_end), 0), num_rows);
+  if (static_cast<int>(blockIdx.x) < clearing) {
+    clear_unnamed(reinterpret_cast<U*>(drows), static_cast<long long>(dim) / kVec, units, token_row, static_cast<long long>(tokens) * k,
+                  num_rows, end, clearing, named_rows);
+    return;
+  }
+  const int block = blockIdx.x - clearing, blocks = gridDim.x - clearing;
+  for (int tb = block * blockDim.y; tb < tokens; tb += blocks * blockDim.y) {
     const int t = tb + threadIdx.y;
     const int* at = token_row + static_cast<long long>(t) * k;
     for (int j = 0; j < k; ++j) {
@@ -465,7 +519,7 @@ combine_backward_kernel(const T* __restrict__ dy, long long ld_dy, const T* __re
 #pragma unroll
             for (int i = 0; i < kVec; ++i) dot = fmaf(to_f32<T>(g.v[i]), to_f32<T>(in.v[i]), dot);
           }
-          if (drows != nullptr) {
+          if (drows != nullptr && r < end) {
             U out;
 #pragma unroll
             for (int i = 0; i < kVec; ++i) out.v[i] = from_f32<T>(w * to_f32<T>(g.v[i]));
@@ -489,13 +543,9 @@ combine_backward_kernel(const T* __restrict__ dy, long long ld_dy, const T* __re
     }
   }
   if (drows != nullptr) {
-    const int end = min(max(*row_end, 0), num_rows);
-    U zero;
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) zero.v[i] = from_f32<T>(0.0f);
-    for (int r = end + blockIdx.x * blockDim.y + threadIdx.y; r < num_rows; r += gridDim.x * blockDim.y)
+    for (int r = end + block * blockDim.y + threadIdx.y; r < num_rows; r += blocks * blockDim.y)
       for (int u = threadIdx.x; u < units; u += blockDim.x)
-        *reinterpret_cast<U*>(drows + static_cast<long long>(r) * dim + static_cast<long long>(u) * kVec) = zero;
+        *reinterpret_cast<U*>(drows + static_cast<long long>(r) * dim + static_cast<long long>(u) * kVec) = U{};
   }
 }
 

@@ -31,6 +31,10 @@ class Routing(NamedTuple):
     offsets:   ``[num_experts + 1]`` int32: first expert-sorted row of every expert, and the end of the last.
     row_token: ``[tokens * top_k]`` int32: the token of every row, -1 from ``offsets[-1]`` on.
     token_row: ``[tokens, top_k]`` int32: the row of every choice, -1 where there was none.
+
+    ``dispatch`` and ``combine`` read ``token_row``, the weights and the end of ``offsets``; a plan of the caller's own needs
+    those, with no row named twice.  A choice whose ``token_row`` is set to -1 (over an expert's capacity, say) is dropped: its
+    row stays the expert's, holds zeros, and adds nothing to the token or to a gradient of the weights behind it.
     """
     weights: Tensor
     experts: Tensor
@@ -218,7 +222,7 @@ class CombineAutoGrad(torch.autograd.Function):
 def dispatch(input: Tensor, routing: Routing) -> Tensor:
     """
     Copies every token's row to its experts: ``[tokens, dim]`` -> ``[tokens * top_k, dim]`` in expert order, zeros in
-    the rows from ``routing.offsets[-1]`` on.
+    all rows that ``routing.token_row`` does not name and in those from ``routing.offsets[-1]`` on.
     """
     assert input.ndim == 2, f'Inputs must be 2D, received shape {input.shape}'
     _require_cuda(input, 'input')

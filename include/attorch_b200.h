@@ -528,8 +528,9 @@ int ab200_route_backward(const void* logits, const float* weights, const int* ch
                          int renormalize, void* stream);
 
 /*
- * rows_out[token_row[t, j]] = x[t]; zeros in the rows from *row_end (offsets[experts]) on.  x: [tokens, dim] of
- * `dtype`, pitch ld_x; rows_out: dense [rows, dim].  Entries of token_row outside [0, rows) are skipped.
+ * rows_out[token_row[t, j]] = x[t]; zeros in all other rows, and in the rows from *row_end (offsets[experts]) on.  x:
+ * [tokens, dim] of `dtype`, pitch ld_x; rows_out: dense [rows, dim].  Entries of token_row outside [0, *row_end) are
+ * skipped, which is how a choice is dropped.  No row may be named twice.
  */
 int ab200_expert_dispatch(const void* x, const int* token_row, const int* row_end, void* rows_out, int64_t tokens, int64_t top_k,
                           int64_t rows, int64_t dim, int64_t ld_x, int dtype, void* stream);
@@ -542,8 +543,8 @@ int ab200_expert_combine(const void* rows_in, const int* token_row, const float*
                          int64_t rows, int64_t dim, int64_t ld_rows, int dtype, void* stream);
 
 /*
- * rows_grad[token_row[t, j]] = weights[t, j] dy[t] (dense [rows, dim]; zeros from *row_end on) and
- * weights_grad[t, j] = <dy[t], rows_in[token_row[t, j]]> (fp32); either may be NULL.
+ * rows_grad[token_row[t, j]] = weights[t, j] dy[t] (dense [rows, dim]; zeros in all other rows, and from *row_end on) and
+ * weights_grad[t, j] = <dy[t], rows_in[token_row[t, j]]> (fp32); either may be NULL.  No row may be named twice.
  */
 int ab200_expert_combine_backward(const void* dy, const void* rows_in, const int* token_row, const float* weights, const int* row_end,
                                   void* rows_grad, float* weights_grad, int64_t tokens, int64_t top_k, int64_t rows, int64_t dim,

@@ -29,3 +29,86 @@ def test_plan_can_be_edited_before_backward(tokens):
     routing.row_token.zero_()
     rows.sum().backward()
     assert torch.equal(x.grad, torch.full_like(x, 2.0))
+
+
+def drop(routing, share, seed):
+    """The plan with a share of its choices dropped, and which choices are left."""
+    g = torch.Generator(device='cuda').manual_seed(seed)
+    keep = (torch.rand(routing.token_row.shape, generator=g, device='cuda') >= share) & (routing.token_row >= 0)
+    return routing._replace(token_row=torch.where(keep, routing.token_row, -1)), keep
+
+
+def poison(*shape, dtype):
+    """Memory that is handed out next holds NaN."""
+    torch.full(shape, float('nan'), dtype=dtype, device='cuda')
+
+
+@pytest.mark.parametrize('tokens,k,dim', [(1, 1, 8), (8, 4, 264), (33, 2, 7), (700, 3, 40), (9000, 8, 16), (1100000, 8, 1)])
+@pytest.mark.parametrize('share', [0.0, 0.3, 1.0])
+def test_dropped_choices_leave_zeros(tokens, k, dim, share):
+    g = torch.Generator(device='cuda').manual_seed(tokens)
+    logits = torch.randn(tokens, max(k, 8), generator=g, device='cuda')
+    mask = torch.rand(tokens, generator=g, device='cuda') >= 0.1
+    routing, keep = drop(attorch.route(logits, k, mask=mask), share, 2)
+    x = torch.randn(tokens, dim, generator=g, device='cuda').bfloat16().requires_grad_()
+    token, row = keep.nonzero()[:, 0], routing.token_row[keep].long()
+    expected = torch.zeros(tokens * k, dim, dtype=x.dtype, device='cuda')
+    expected[row] = x.detach()[token]
+    poison(tokens * k, dim, dtype=x.dtype)
+    rows = attorch.dispatch(x, routing)
+    assert torch.equal(rows, expected)
+    drows = torch.randn(tokens * k, dim, generator=g, device='cuda').bfloat16()
+    poison(tokens, dim, dtype=x.dtype)
+    dx, = torch.autograd.grad(rows, x, drows)
+    total = torch.zeros(tokens, dim, dtype=torch.float64, device='cuda').index_add_(0, token, drows[row].double())
+    size = torch.zeros(tokens, dim, dtype=torch.float64, device='cuda').index_add_(0, token, drows[row].double().abs())
+    assert ((dx.double() - total).abs() <= 2.0 ** -9 * 2 * total.abs() + k * 2.0 ** -23 * size).all()
+
+    h = torch.randn(tokens * k, dim, generator=g, device='cuda').bfloat16().requires_grad_()
+    weights = routing.weights.detach().requires_grad_()
+    dy = torch.randn(tokens, dim, generator=g, device='cuda').bfloat16()
+    y = attorch.combine(h, routing._replace(weights=weights))
+    poison(tokens * k, dim, dtype=x.dtype)
+    dh, dw = torch.autograd.grad(y, (h, weights), dy)
+    # A weight times a gradient is rounded to fp32 before it is stored: two roundings.
+    dh64 = torch.zeros(tokens * k, dim, dtype=torch.float64, device='cuda')
+    dh64[row] = weights.detach()[keep].double()[:, None] * dy[token].double()
+    assert ((dh.double() - dh64).abs() <= (2.0 ** -9 * 2 + 2.0 ** -23) * dh64.abs()).all()
+    products = h.detach()[row].double() * dy[token].double()
+    assert not dw[~keep].any()
+    assert ((dw[keep].double() - products.sum(1)).abs() <= dim * 2.0 ** -23 * products.abs().sum(1)).all()
+
+
+def test_rows_behind_the_end_are_zeros_whatever_names_them():
+    """A plan cut off at a smaller end: no entry reaches behind it."""
+    routing = attorch.route(torch.randn(300, 4, device='cuda'), 2)
+    routing.offsets.clamp_(max=201)
+    x = torch.randn(300, 64, device='cuda')
+    for _ in range(20):
+        rows = attorch.dispatch(x, routing)
+        assert not rows[201:].any() and torch.equal(rows[:201], x[routing.row_token[:201].long()])
+        h = torch.ones(600, 64, device='cuda', requires_grad=True)
+        attorch.combine(h, routing).sum().backward()
+        assert not h.grad[201:].any() and (h.grad[:201] > 0).all()
+
+
+def test_block_trains_with_dropped_choices():
+    """Choices over a capacity dropped between routing and the experts: as if their rows did not exist."""
+    torch.manual_seed(3)
+    block = attorch.MixtureOfExperts(64, 96, 4, 2, 'silu', dtype=torch.bfloat16)
+    x = torch.randn(400, 64, device='cuda').bfloat16()
+    poisoned = []
+    for again in range(2):
+        routing, keep = drop(block.router(x), 0.4, 4)
+        if again:
+            for width in (64, 96):
+                poison(800, width, dtype=x.dtype)
+        rows = block.down(block.up(attorch.dispatch(x, routing), routing.offsets), routing.offsets)
+        y = attorch.combine(rows, routing)
+        if again:
+            for width in (64, 96):
+                poison(800, width, dtype=x.dtype)
+        poisoned.append((y, *torch.autograd.grad(y, [block.up.weight, block.up.bias, block.down.weight, block.down.bias], torch.ones_like(y))))
+    assert all(torch.isfinite(t).all() for t in poisoned[0]) and int((~keep).sum()) > 200
+    for a, b in zip(*poisoned):
+        assert torch.equal(a, b)
