@@ -54,6 +54,13 @@ def _inner_unit(tensor: Tensor) -> Tensor:
 _SCORE_FUNCS = {'softmax': 0, 'sigmoid': 1}
 
 
+def _check_mask(mask: Optional[Tensor], tokens: int, device: torch.device) -> None:
+    if mask is not None:
+        assert mask.shape == (tokens,), f'The mask must have one entry per token ({tokens}), received shape {mask.shape}'
+        assert mask.dtype is torch.bool, f'The mask must be boolean, received {mask.dtype}'
+        assert mask.device == device, f'The mask is on {mask.device}, the tokens on {device}'
+
+
 def _route(logits: Tensor, top_k: int, score_func: str, renormalize: bool, mask: Optional[Tensor], needs_grad: bool):
     assert logits.ndim == 2, f'Logits must be 2D, received shape {logits.shape}'
     tokens, experts = logits.shape
@@ -64,10 +71,8 @@ def _route(logits: Tensor, top_k: int, score_func: str, renormalize: bool, mask:
         f'top_k must be 1 to {min(experts, MAX_TOP_K)} for {experts} experts, received {top_k}'
     _require_cuda(logits, 'logits')
     device = logits.device
+    _check_mask(mask, tokens, device)
     if mask is not None:
-        assert mask.shape == (tokens,), f'The mask must have one entry per token ({tokens}), received shape {mask.shape}'
-        assert mask.dtype is torch.bool, f'The mask must be boolean, received {mask.dtype}'
-        assert mask.device == device, f'The mask is on {mask.device}, the logits on {device}'
         mask = mask if mask.is_contiguous() else mask.contiguous()
     dtype = _dtype_id(logits.dtype)
     logits = _inner_unit(logits)
@@ -131,7 +136,7 @@ def route(logits: Tensor, top_k: int, score_func: str = 'softmax', renormalize: 
         top_k: Experts a token, at most 32.
         score_func: 'softmax' (over all experts) or 'sigmoid': the weight of a chosen expert.
         renormalize: Flag for dividing a token's weights by their sum.
-        mask: Optional ``[tokens]`` boolean; False (padding) sends a token to no expert.
+        mask: Optional ``[tokens]`` boolean; False (padding) sends a token to no expert, whatever its logits are.
     """
     if recorded(logits):
         return Routing(*RouteAutoGrad.apply(logits, top_k, score_func, renormalize, mask))
@@ -259,15 +264,17 @@ class GateAutoGrad(torch.autograd.Function):
     ``apply(input, weight)``: ``input @ weight`` with the bits of a row independent of timing.  ``Linear`` shares the
     reduction of a product this narrow out over all SMs and adds the pieces atomically, in an order that changes
     from call to call; a token whose logits nearly tie could then change its experts.  The grouped kernel with one
-    group sums every output in one place.  Backward is ``Linear``'s, and the optional trailing arguments are those of
-    ``LinearAutoGrad`` for data-parallel training (where ``dW`` goes, who is told, what is put off).
+    group sums every output in one place.  Backward is ``Linear``'s, but rows where ``mask`` is False stay
+    out of ``dW`` whatever they hold (their logits have no gradient, and zero times NaN is NaN).  The optional trailing
+    arguments are those of ``LinearAutoGrad`` for data-parallel training (where ``dW`` goes, who is told, what is put off).
     """
     @staticmethod
-    def forward(ctx, input: Tensor, weight: Tensor, weight_grad_out: Optional[Tensor] = None, grad_ready=None,
-                dw_chunks: int = 1, defer_input_grad=None) -> Tensor:
+    def forward(ctx, input: Tensor, weight: Tensor, mask: Optional[Tensor] = None, weight_grad_out: Optional[Tensor] = None,
+                grad_ready=None, dw_chunks: int = 1, defer_input_grad=None) -> Tensor:
         assert input.ndim == 2 and input.shape[1] == weight.shape[0], \
             f'Incompatible input ({input.shape}) and weights ({weight.shape}) shape'
         assert weight.device == input.device, f'The weights are on {weight.device}, the input on {input.device}'
+        _check_mask(mask, input.shape[0], input.device)
         _require_cuda(input, 'input')
         _require_cuda(weight, 'weight')
         rows, in_dim = input.shape
@@ -287,12 +294,12 @@ class GateAutoGrad(torch.autograd.Function):
         ctx.needs = (input.requires_grad, weight.requires_grad)
         ctx.weight_grad_out, ctx.grad_ready, ctx.dw_chunks = weight_grad_out, grad_ready, int(dw_chunks)
         ctx.defer_input_grad = defer_input_grad
-        ctx.save_for_backward(x_op, w_op)
+        ctx.save_for_backward(x_op, w_op, mask)
         return output
 
     @staticmethod
     def backward(ctx, output_grad: Tensor) -> Tuple[Optional[Tensor], ...]:
-        x_op, w_op = ctx.saved_tensors
+        x_op, w_op, mask = ctx.saved_tensors
         rows, in_dim = x_op.shape
         experts, dtype, device = w_op.shape[1], x_op.dtype, x_op.device
         dt = _dtype_id(dtype)
@@ -300,6 +307,8 @@ class GateAutoGrad(torch.autograd.Function):
         with on(device):
             dy = _rows_operand(output_grad, dtype, stream_of(device))
             if ctx.needs[1]:
+                if mask is not None:
+                    x_op = _rows_operand(x_op.masked_fill(~mask[:, None], 0), dtype, stream_of(device))
                 weight_grad = ctx.weight_grad_out if ctx.weight_grad_out is not None else \
                     torch.empty((in_dim, experts), dtype=ctx.dtypes[1], device=device)
                 # Blocks of rows of dW, each handed to the gradient exchange as soon as it is enqueued.
@@ -332,7 +341,7 @@ class GateAutoGrad(torch.autograd.Function):
                 else:
                     launch_input_grad()
         # A gradient that went to the caller's buffer is not returned as well: autograd would add it to ``.grad``.
-        return input_grad, None if ctx.weight_grad_out is not None else weight_grad, None, None, None, None
+        return input_grad, None if ctx.weight_grad_out is not None else weight_grad, None, None, None, None, None
 
 
 def _gemm_workspace(device: torch.device, *shape: int) -> Tuple[Optional[Tensor], int]:
@@ -377,5 +386,6 @@ class Router(nn.Module):
     def forward(self, input: Tensor, mask: Optional[Tensor] = None) -> Routing:
         """``input``: ``[tokens, dim]``; ``mask``: see ``route``."""
         gate = self.gate
-        logits = GateAutoGrad.apply(input, gate.weight, gate.weight_grad_out, gate.grad_ready, gate.dw_chunks, gate.defer_input_grad)
+        logits = GateAutoGrad.apply(input, gate.weight, mask, gate.weight_grad_out, gate.grad_ready, gate.dw_chunks,
+                                    gate.defer_input_grad)
         return route(logits, self.top_k, self.score_func, self.renormalize, mask)

@@ -49,7 +49,8 @@ class MixtureOfExperts(nn.Module):
         return self
 
     def forward(self, input: Tensor, mask: Optional[Tensor] = None) -> Tensor:
-        """``input``: ``[..., dim]``; ``mask``: optional ``[...]`` boolean, False for padding, whose output is zero."""
+        """``input``: ``[..., dim]``; ``mask``: optional ``[...]`` boolean, False for padding, whose output is
+        zero and whose values, NaN among them, reach no gradient of the parameters."""
         tokens = input.flatten(0, -2)
         routing = self.router(tokens, None if mask is None else mask.flatten())
         rows = self.up(dispatch(tokens, routing), routing.offsets)

@@ -112,3 +112,29 @@ def test_block_trains_with_dropped_choices():
     assert all(torch.isfinite(t).all() for t in poisoned[0]) and int((~keep).sum()) > 200
     for a, b in zip(*poisoned):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('gated', [False, True])
+@pytest.mark.parametrize('held', [float('nan'), float('inf')])
+@pytest.mark.parametrize('dim', [64, 60])
+def test_padding_may_hold_anything(gated, held, dim):
+    """Fully masked attention rows are NaN: as padding they change no output, gradient or parameter's gradient."""
+    torch.manual_seed(5)
+    block = attorch.MixtureOfExperts(dim, 96, 4, 2, 'gelu', gated=gated, dtype=torch.bfloat16)
+    x = torch.randn(4, 50, dim, device='cuda').bfloat16()
+    mask = torch.rand(4, 50, device='cuda') >= 0.3
+    dy = torch.randn(4, 50, dim, device='cuda').bfloat16()
+    results = []
+    for value in (0.0, held):
+        xx = torch.where(mask[..., None], x, value).requires_grad_()
+        y = block(xx, mask)
+        results.append((y, *torch.autograd.grad(y, [xx, *block.parameters()], dy)))
+    names = ('y', 'x', *(name for name, _ in block.named_parameters()))
+    for name, a, b in zip(names, *results):
+        assert torch.isfinite(b).all(), name
+        if name in ('x', 'router.gate.weight'):        # Linear's products: their pieces may be added in another order
+            torch.testing.assert_close(a, b, rtol=2.0 ** -7, atol=2.0 ** -7)
+        else:
+            assert torch.equal(a, b), name
+    assert not results[1][0][~mask].any() and not results[1][1][~mask].any()
+    attorch.check_status()
