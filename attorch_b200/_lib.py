@@ -26,6 +26,7 @@ FLAG_SAVE_DERIVATIVE = 64
 FLAG_WHOLE_TILES = 128
 FLAG_DROPOUT_PACKED = 256
 FLAG_DERIVATIVE_FP16 = 512
+FLAG_OUTPUT_FP32 = 1024
 FLAG_RESERVE_SMS_SHIFT = 16   # bits 16-23: SMs a GEMM call leaves free
 ACT_NONE = 0
 ACT_SAVED_DERIVATIVE = 22

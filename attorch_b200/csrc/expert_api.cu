@@ -146,6 +146,7 @@ int ab200_grouped_linear_forward(const void* x, const void* w, const void* bias,
   int rc = check_grouped(rows, groups, K, N);
   if (rc != OK) return rc;
   if (!valid_dtype(dtype) || (bias && !valid_dtype(bias_dtype))) return ERR_BAD_DTYPE;
+  if ((flags & AB200_FLAG_OUTPUT_FP32) && pre_act) return ERR_BAD_DTYPE;
   if (!valid_act(act)) return ERR_BAD_ACT;
   if (offsets == nullptr && groups != 1) return ERR_NULL_POINTER;
   if (rows == 0 || N == 0) return OK;
@@ -157,12 +158,12 @@ int ab200_grouped_linear_forward(const void* x, const void* w, const void* bias,
   g.offsets = offsets;
   g.groups = static_cast<int>(groups); g.rows = static_cast<int>(rows);
   g.N = static_cast<int>(N); g.K = static_cast<int>(K);
-  g.out = out; g.ld_out = ld_out; g.out_dtype = dtype;
+  g.out = out; g.ld_out = ld_out; g.out_dtype = (flags & AB200_FLAG_OUTPUT_FP32) ? static_cast<int>(DT_F32) : dtype;
   g.aux = pre_act; g.ld_aux = ld_pre;
   g.bias = bias; g.bias_dtype = bias_dtype;
   g.act = act; g.act_param = act_param;
   g.save_grad = (flags & AB200_FLAG_SAVE_DERIVATIVE) && act != ACT_NONE ? 1 : 0;
-  g.grad_dtype = g.save_grad && dtype == DT_BF16 && (flags & AB200_FLAG_DERIVATIVE_FP16) ? DT_F16 : dtype;
+  g.grad_dtype = g.save_grad && dtype == DT_BF16 && (flags & AB200_FLAG_DERIVATIVE_FP16) ? DT_F16 : g.out_dtype;
   const bool tc_ok = K > 0 && aligned16(x, ld_x, elt) && aligned16(w, ld_w, elt) && w_group_stride * elt % 16 == 0;
   if ((flags & AB200_FLAG_FORCE_TCGEN05) && !tc_ok) return ERR_BAD_STRIDE;
   if (!tc_ok || (flags & AB200_FLAG_FORCE_GENERIC)) {

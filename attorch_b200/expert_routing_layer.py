@@ -264,7 +264,8 @@ class GateAutoGrad(torch.autograd.Function):
     ``apply(input, weight)``: ``input @ weight`` with the bits of a row independent of timing.  ``Linear`` shares the
     reduction of a product this narrow out over all SMs and adds the pieces atomically, in an order that changes
     from call to call; a token whose logits nearly tie could then change its experts.  The grouped kernel with one
-    group sums every output in one place.  Backward is ``Linear``'s, but rows where ``mask`` is False stay
+    group sums every output in one place.  The logits are fp32 whatever type is multiplied (fp32 as TF32, as in ``Linear``):
+    rounded to 16 bits, near ties would become ties, which the lowest index wins.  Backward is ``Linear``'s, but rows where ``mask`` is False stay
     out of ``dW`` whatever they hold (their logits have no gradient, and zero times NaN is NaN).  The optional trailing
     arguments are those of ``LinearAutoGrad`` for data-parallel training (where ``dW`` goes, who is told, what is put off).
     """
@@ -285,11 +286,11 @@ class GateAutoGrad(torch.autograd.Function):
             stream = stream_of(input.device)
             x_op = _rows_operand(input, dtype, stream)
             w_op = _rows_operand(weight, dtype, stream)
-            output = torch.empty((rows, experts), dtype=dtype, device=input.device)
+            output = torch.empty((rows, experts), dtype=torch.float32, device=input.device)
             _lib.check(lib.ab200_grouped_linear_forward(
                 _ptr(x_op), _ptr(w_op), None, None, None, _ptr(output), rows, 1, in_dim, experts, _pitch(x_op), 0, _pitch(w_op),
                 experts, experts, _dtype_id(dtype), 0, _lib.ACT_NONE, 0.0, status_of(input.device), stream,
-                _flags_for(input.device)), 'ab200_grouped_linear_forward')
+                _flags_for(input.device) | _lib.FLAG_OUTPUT_FP32), 'ab200_grouped_linear_forward')
         ctx.dtypes = (input.dtype, weight.dtype)
         ctx.needs = (input.requires_grad, weight.requires_grad)
         ctx.weight_grad_out, ctx.grad_ready, ctx.dw_chunks = weight_grad_out, grad_ready, int(dw_chunks)
@@ -305,6 +306,7 @@ class GateAutoGrad(torch.autograd.Function):
         dt = _dtype_id(dtype)
         input_grad = weight_grad = None
         with on(device):
+            # The gradient of the logits is rounded to the operands' type here, for the tensor cores.
             dy = _rows_operand(output_grad, dtype, stream_of(device))
             if ctx.needs[1]:
                 if mask is not None:

@@ -100,6 +100,7 @@ extern "C" {
 #define AB200_FLAG_DERIVATIVE_FP16 512 /* forward with SAVE_DERIVATIVE and a bf16 output: act'(Z) is stored
                                         * as fp16 (same size, 3 more mantissa bits; derivatives are O(1)), so
                                         * that dZ = dY * act'(Z) is in effect rounded once, as the reference's */
+#define AB200_FLAG_OUTPUT_FP32 1024 /* ab200_grouped_linear_forward without pre_act: out is fp32 whatever `dtype` is */
 /* Bits 16-23 of the flags of a GEMM entry point: the number of SMs (0-255) the persistent kernel of
  * that call leaves free, for a collective that runs beside it (same purpose as
  * ab200_set_gemm_cta_limit, but per call instead of process-wide). */
@@ -470,10 +471,10 @@ int ab200_layer_norm_backward(const void* dy, const void* x, const float* mean, 
  *   pre_act  [rows, N] or NULL: the value before the activation, or act'(Z) with AB200_FLAG_SAVE_DERIVATIVE
  *            (and AB200_FLAG_DERIVATIVE_FP16), as ab200_linear_forward, but at the fp32 Z: there is no form of
  *            these operators elsewhere whose rounding of Z to `dtype` would have to be matched
- *   out      [rows, N] of `dtype`
+ *   out      [rows, N] of `dtype`, or of fp32 with AB200_FLAG_OUTPUT_FP32 (AB200_ERR_BAD_DTYPE if pre_act is given too)
  * fp32 operands are multiplied as TF32.  Operands that are not 16-byte aligned, or whose pitches are no multiples
  * of 16 bytes, run on a CUDA-core kernel.  status is required.  flags: AB200_FLAG_FORCE_GENERIC,
- * AB200_FLAG_FORCE_TCGEN05, AB200_FLAG_NO_PAIR, AB200_FLAG_NO_TMA_STORE, AB200_FLAG_RESERVE_SMS(n).
+ * AB200_FLAG_FORCE_TCGEN05, AB200_FLAG_OUTPUT_FP32, AB200_FLAG_NO_PAIR, AB200_FLAG_NO_TMA_STORE, AB200_FLAG_RESERVE_SMS(n).
  */
 int ab200_grouped_linear_forward(const void* x, const void* w, const void* bias, const int* offsets, void* pre_act, void* out,
                                  int64_t rows, int64_t groups, int64_t K, int64_t N, int64_t ld_x, int64_t w_group_stride,

@@ -59,3 +59,15 @@ def test_frozen_copies_leave_the_trained_layer_alone(monkeypatch):
         with torch.no_grad():
             source.bias.add_(1.0)
         assert torch.equal(copy.bias, before)
+
+
+def test_fp32_output_excludes_a_kept_pre_activation():
+    from attorch_b200 import _lib
+    from attorch_b200 import build as builder
+    builder.build()
+    a = 0x1000
+    for dtype in (_lib.F32, _lib.F16, _lib.BF16):
+        assert _lib.load().ab200_grouped_linear_forward(a, a, None, None, a, a, 0, 1, 8, 8, 8, 0, 8, 8, 8, dtype, 0, 0, 0.0, a, None,
+                                                        _lib.FLAG_OUTPUT_FP32) == -3
+        assert _lib.load().ab200_grouped_linear_forward(a, a, None, None, None, a, 0, 1, 8, 8, 8, 0, 8, 8, 8, dtype, 0, 0, 0.0, a, None,
+                                                        _lib.FLAG_OUTPUT_FP32) == 0

@@ -70,3 +70,36 @@ def test_gate_tells_the_exchange_and_puts_its_input_gradient_off():
     gate_step(router, x, dweights)
     assert [t[:2] for t in told] == [(0, 1)]
     attorch.check_status()
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize('tokens,dim,experts', [(3, 64, 8), (300, 100, 12), (40, 4096, 130)])
+def test_logits_are_fp32(dtype, tokens, dim, experts):
+    """Products of 16-bit operands summed in fp32 and not rounded: off by at most dim 2^-23 of the sum of magnitudes."""
+    from attorch_b200.expert_routing_layer import GateAutoGrad
+    g = torch.Generator(device='cuda').manual_seed(dim)
+    x = torch.randn(tokens, dim, generator=g, device='cuda').to(dtype).requires_grad_()
+    w = torch.randn(dim, experts, generator=g, device='cuda').to(dtype).requires_grad_()
+    logits = GateAutoGrad.apply(x, w)
+    expected, size = x.detach().double() @ w.detach().double(), x.detach().double().abs() @ w.detach().double().abs()
+    assert logits.dtype is torch.float32 and ((logits.double() - expected).abs() <= dim * 2.0 ** -23 * size).all()
+    dlogits = torch.randn(tokens, experts, generator=g, device='cuda').to(dtype)      # exact in the operands' type
+    dx, dw = torch.autograd.grad(logits, (x, w), dlogits.float())
+    eps = torch.finfo(dtype).eps / 2
+    for got, left, right in ((dx, dlogits, w.detach().T), (dw, x.detach().T, dlogits)):
+        exact, size = left.double() @ right.double(), left.double().abs() @ right.double().abs()
+        assert got.dtype is dtype
+        assert ((got.double() - exact).abs() <= eps * exact.abs() + 1.1 * left.shape[1] * 2.0 ** -23 * size + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize('dtype,gap', [(torch.bfloat16, 2.0 ** -10), (torch.float16, 2.0 ** -13), (torch.float32, 2.0 ** -9)], ids=str)
+def test_near_ties_go_to_the_larger_logit(dtype, gap):
+    """1 and 1 + gap are one number in 16 bits; the second expert's logit is larger."""
+    router = attorch.Router(16, 4, 1, dtype=dtype)
+    with torch.no_grad():
+        router.gate.weight.zero_()
+        router.gate.weight[0, :3] = 1.0
+        router.gate.weight[1, 1] = 1.0
+        x = torch.zeros(5, 16, device='cuda', dtype=dtype)
+        x[:, 0], x[:, 1] = 1.0, gap
+        assert (router(x).experts == 1).all()
