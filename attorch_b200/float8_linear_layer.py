@@ -211,12 +211,14 @@ class Float8LinearAutoGrad(torch.autograd.Function):
         out_dtype = get_output_dtype(input.dtype)
         with on(input.device):
             stream = stream_of(input.device)
-            x_op = _rows_operand(flat, out_dtype, stream)
+            x_op = _rows_operand(flat, out_dtype, stream) if ctx.needs[1] else None
             output = torch.empty((rows, out_dim), dtype=out_dtype, device=input.device)
             wq = scale = kept = None
             ctx.backward_act = (_lib.ACT_NONE, 0.0)
             if output.numel():
-                xq, x_scale = _quantize_rows(x_op, stream)
+                # From the values as they came, like a stored weight's product: rounded to 16 bits first (under autocast), some
+                # would be held as a neighbour, and the frozen layer would differ from the one that was trained.
+                xq, x_scale = _quantize_rows(x_op if x_op is not None and flat.dtype is out_dtype else flat, stream)
                 wq, wq_t, scale = _quantize_weight(weight, ctx.needs[0], True, stream)
                 kept, flags, ctx.backward_act = _kept_for_backward(name, param, out_dtype, (rows, out_dim), input.device, any(ctx.needs))
                 bias_op = bias if bias is None or bias.is_contiguous() else bias.contiguous()
@@ -225,7 +227,7 @@ class Float8LinearAutoGrad(torch.autograd.Function):
         ctx.shapes = (input.shape, rows, in_dim, out_dim)
         ctx.dtypes = (input.dtype, weight.dtype, None if bias is None else bias.dtype)
         if any(ctx.needs):
-            ctx.save_for_backward(x_op if ctx.needs[1] else None, wq, scale, kept)
+            ctx.save_for_backward(x_op, wq, scale, kept)
         return output.view(*input.shape[:-1], out_dim)
 
     @staticmethod

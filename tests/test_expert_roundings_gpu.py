@@ -113,3 +113,27 @@ def test_pre_activation_is_kept_where_the_caller_asks(act, dtype, rows, n, eight
     expected = torch.stack([x[r].double().T @ dz[r] for _, r in groups]).view_as(leaf)
     bound = torch.stack([x[r].double().abs().T @ (size[r] + rows * 2.0 ** -23 * dz[r].abs()) for _, r in groups]).view_as(leaf)
     assert ((dw.double() - expected).abs() <= bound + eps * (expected.abs() + bound)).all()
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize('rows,k,n', [(70, 256, 136), (33, 100, 72)])
+def test_frozen_layer_gives_the_trained_ones_bits_under_autocast(dtype, rows, k, n):
+    """Both quantise the fp32 input itself; so the training form is right with respect to its held value too."""
+    from tests.expert_helpers import held_as_e4m3
+    torch.manual_seed(1)
+    layer = attorch.Float8Linear(k, n, act_func='silu')
+    x = torch.randn(rows, k, device='cuda')
+    wide = torch.randn(rows, k + 3, device='cuda')
+    for xx in (x, wide[:, 3:], x.T.contiguous().T):
+        with torch.autocast('cuda', dtype=dtype):
+            trained = layer(xx.clone().requires_grad_() if xx is x else xx)
+            with torch.no_grad():
+                evaluated = layer(xx)
+                weight, scale = attorch.quantize_weight(layer.weight)
+                served = attorch.float8_linear(xx, weight, scale, layer.bias, 'silu')
+        assert trained.dtype is dtype and torch.equal(trained, served) and torch.equal(evaluated, served)
+    z = held_as_e4m3(x, 1)[0] @ held_as_e4m3(layer.weight.detach(), 128)[0]
+    size = held_as_e4m3(x, 1)[0].abs() @ held_as_e4m3(layer.weight.detach(), 128)[0].abs()
+    with torch.autocast('cuda', dtype=dtype), torch.no_grad():
+        plain = attorch.Float8LinearAutoGrad.apply(x, layer.weight, None, None)
+    assert ((plain.double() - z).abs() <= torch.finfo(dtype).eps / 2 * z.abs() + k * 2.0 ** -23 * size + 2.0 ** -25).all()
