@@ -33,6 +33,7 @@ ACT_SAVED_DERIVATIVE = 22
 ACT_SAVED_DERIVATIVE_F16 = 23
 
 PATH_TCGEN05, PATH_STREAMK, PATH_GENERIC = 1, 2, 3
+TILE_PAIR = 0x1000
 
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
@@ -45,6 +46,7 @@ SIGNATURES = {
     'ab200_error_string': (ctypes.c_char_p, [_int]),
     'ab200_last_path': (_int, []),
     'ab200_last_schedule': (_int, []),
+    'ab200_last_tile': (_int, []),
     'ab200_launch_count': (_i64, []),
     'ab200_set_gemm_cta_limit': (_int, [_int]),
     'ab200_forward_workspace_bytes': (_i64, [_i64, _i64, _i64, _int]),

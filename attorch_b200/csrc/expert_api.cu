@@ -13,6 +13,9 @@
 
 namespace ab200 {
 
+namespace { thread_local int g_last_tile = 0; }
+void set_last_tile(int tile) { g_last_tile = tile; }
+
 int encode_3d(CUtensorMap* map, int elt, const void* base, uint64_t inner, uint64_t rows, uint64_t outer, uint64_t pitch_bytes,
               uint64_t group_bytes, uint32_t box_inner, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
   using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -71,6 +74,8 @@ struct TileCost {
   double cost;
 };
 constexpr TileCost kCosts16[] = {{256, true, 0.42}, {256, false, 0.50}, {128, false, 0.42}, {64, false, 0.38}};
+// fp32 as TF32 has two shapes (18944 x 2048 ... 8192 x 2048, 4 x 9472 x 8192 x 512: 0.39-0.41 and 0.33-0.37).
+constexpr TileCost kCosts32[] = {{256, true, 0.40}, {128, false, 0.35}};
 constexpr TileCost kCosts8[] = {{256, true, 0.65}, {128, false, 0.38}, {64, false, 0.33}, {32, false, 0.31}};
 
 // The shape with the least rounds x cost; equal ones by the order above.  row_tiles(tile_m): expected row tiles of
@@ -91,6 +96,12 @@ Tile pick_tile(const TileCost (&costs)[kCount], int64_t N, bool allow_pair, F&& 
     }
   }
   return best;
+}
+
+// The same among the shapes that the type's kernels have.
+template <class F>
+Tile pick_tile_of(int dtype, int64_t N, bool allow_pair, F&& row_tiles) {
+  return dtype == DT_F32 ? pick_tile(kCosts32, N, allow_pair, row_tiles) : pick_tile(kCosts16, N, allow_pair, row_tiles);
 }
 
 // Ragged rows: the host knows their number but not how they fall into groups.  Every group that can have rows has at
@@ -122,6 +133,7 @@ int launch_any_grouped(const AnyGroupedArgs& a, cudaStream_t stream) {
   if (row_tiles >= (1ll << 31) || (g.N + 63) / 64 > 65535) return ERR_TOO_LARGE;
   grouped_any_kernel<kRagged><<<dim3(static_cast<unsigned>(row_tiles), (g.N + 63) / 64), 256, 0, stream>>>(a);
   set_last_path(AB200_PATH_GENERIC);
+  set_last_tile(0);
   return launched();
 }
 
@@ -137,6 +149,8 @@ int check_grouped(int64_t rows, int64_t groups, int64_t K, int64_t N) {
 using namespace ab200;
 
 extern "C" {
+
+int ab200_last_tile(void) { return g_last_tile; }
 
 int ab200_grouped_linear_forward(const void* x, const void* w, const void* bias, const int* offsets, void* pre_act, void* out,
                                  int64_t rows, int64_t groups, int64_t K, int64_t N, int64_t ld_x, int64_t w_group_stride,
@@ -176,7 +190,7 @@ int ab200_grouped_linear_forward(const void* x, const void* w, const void* bias,
   }
   p.a = x; p.a_pitch = ld_x;
   p.b = w; p.b_pitch = ld_w; p.b_group_pitch = w_group_stride; p.b_rows = g.K; p.b_cols = g.N;
-  const Tile t = pick_tile(kCosts16, N, p.allow_pair, ragged_row_tiles(rows, groups));
+  const Tile t = pick_tile_of(dtype, N, p.allow_pair, ragged_row_tiles(rows, groups));
   set_last_path(AB200_PATH_TCGEN05);
   return dtype == DT_F32 ? launch_grouped_forward_32(p, t.bn, t.pair, stream) : launch_grouped_forward_16(p, t.bn, t.pair, stream);
 }
@@ -210,7 +224,7 @@ int ab200_grouped_linear_backward_input(const void* dz, const void* w, const int
   }
   p.a = dz; p.a_pitch = ld_dz;
   p.b = w; p.b_pitch = ld_w; p.b_group_pitch = w_group_stride; p.b_rows = static_cast<int>(K); p.b_cols = static_cast<int>(N);
-  const Tile t = pick_tile(kCosts16, K, p.allow_pair, ragged_row_tiles(rows, groups));
+  const Tile t = pick_tile_of(dtype, K, p.allow_pair, ragged_row_tiles(rows, groups));
   set_last_path(AB200_PATH_TCGEN05);
   return dtype == DT_F32 ? launch_grouped_input_32(p, t.bn, t.pair, stream) : launch_grouped_input_16(p, t.bn, t.pair, stream);
 }
@@ -248,7 +262,7 @@ int ab200_grouped_linear_backward_weight(const void* x, const void* dz, const in
   p.a = x; p.a_pitch = ld_x;
   p.b = dz; p.b_pitch = ld_dz;
   // Every weight has the same tiles.
-  const Tile t = pick_tile(kCosts16, N, p.allow_pair, [=](int tile_m) { return groups * ((K + tile_m - 1) / tile_m); });
+  const Tile t = pick_tile_of(dtype, N, p.allow_pair, [=](int tile_m) { return groups * ((K + tile_m - 1) / tile_m); });
   set_last_path(AB200_PATH_TCGEN05);
   return dtype == DT_F32 ? launch_grouped_weight_32(p, t.bn, t.pair, stream) : launch_grouped_weight_16(p, t.bn, t.pair, stream);
 }

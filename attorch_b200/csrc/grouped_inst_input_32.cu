@@ -4,6 +4,7 @@
 namespace ab200 {
 int launch_grouped_input_32(const GroupedProblem& p, int bn, bool pair, cudaStream_t stream) {
   if (pair) return launch_grouped_cfg<GroupedCfg<256, 4, false, false, 2>>(p, stream);
-  return launch_grouped_cfg<GroupedCfg<128, 4, false, false>>(p, stream);
+  if (bn == 128) return launch_grouped_cfg<GroupedCfg<128, 4, false, false>>(p, stream);
+  return ERR_BAD_SHAPE;
 }
 }  // namespace ab200

@@ -6,6 +6,7 @@ int launch_grouped_weight_16(const GroupedProblem& p, int bn, bool pair, cudaStr
   if (pair) return launch_grouped_cfg<GroupedCfg<256, 2, true, true, 2>>(p, stream);
   if (bn == 64) return launch_grouped_cfg<GroupedCfg<64, 2, true, true>>(p, stream);
   if (bn == 128) return launch_grouped_cfg<GroupedCfg<128, 2, true, true>>(p, stream);
-  return launch_grouped_cfg<GroupedCfg<256, 2, true, true>>(p, stream);
+  if (bn == 256) return launch_grouped_cfg<GroupedCfg<256, 2, true, true>>(p, stream);
+  return ERR_BAD_SHAPE;
 }
 }  // namespace ab200

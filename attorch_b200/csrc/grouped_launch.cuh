@@ -1,9 +1,10 @@
 // Host side of the grouped products (grouped_gemm.cuh): tensor maps, tile choice and launch.  The kernel
 // families are instantiated in grouped_inst_*.cu; arguments are validated by the C-ABI functions in
-// grouped_api.cu.
+// expert_api.cu.
 #pragma once
 #include <cuda_runtime.h>
 
+#include "../../include/attorch_b200.h"
 #include "gemm_launch.cuh"
 #include "grouped_gemm.cuh"
 
@@ -12,6 +13,8 @@ namespace ab200 {
 // Counts a kernel launched outside api.cu (ab200_launch_count) and names the kernel family of the last call.
 void count_launches(int n);
 void set_last_path(int path);
+// The tile shape that a grouped product launched (ab200_last_tile).
+void set_last_tile(int tile);
 bool cta_pair_allowed(int flags);
 
 struct GroupedProblem {
@@ -30,7 +33,8 @@ struct GroupedProblem {
 int encode_3d(CUtensorMap* map, int elt, const void* base, uint64_t inner, uint64_t rows, uint64_t outer, uint64_t pitch_bytes,
               uint64_t group_bytes, uint32_t box_inner, uint32_t box_rows, CUtensorMapSwizzle swizzle);
 
-// Families; bn in {32 (8-bit), 64, 128, 256 (not 8-bit)}, pairs of CTAs with bn = 256.
+// Families.  Pairs of CTAs have bn = 256; single CTAs 64, 128 or 256 (2-byte types), 128 (fp32), 32, 64 or 128 (8-bit).  A
+// width that a family does not have is an error: what runs is what the tile choice has costed.
 int launch_grouped_forward_16(const GroupedProblem& p, int bn, bool pair, cudaStream_t stream);
 int launch_grouped_input_16(const GroupedProblem& p, int bn, bool pair, cudaStream_t stream);
 int launch_grouped_weight_16(const GroupedProblem& p, int bn, bool pair, cudaStream_t stream);
@@ -129,6 +133,7 @@ int launch_grouped_cfg(const GroupedProblem& p, cudaStream_t stream) {
   cfg.gridDim = dim3(workers * Cfg::CTAS);
   cfg.stream = stream;
   if (cudaLaunchKernelEx(&cfg, grouped_gemm_kernel<Cfg>, ta, ta_box, tb, tout, taux, g) != cudaSuccess) return ERR_LAUNCH;
+  set_last_tile(Cfg::BN | (Cfg::CTAS > 1 ? AB200_TILE_PAIR : 0));
   count_launches(1);
   return OK;
 }

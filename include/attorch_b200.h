@@ -129,6 +129,11 @@ int ab200_last_path(void);
  */
 int ab200_last_schedule(void);
 
+/* Columns of the tile that the last grouped or 8-bit product launched from this host thread ran with, and whether pairs
+ * of CTAs shared it (AB200_TILE_PAIR); 0 after one on CUDA cores.  For tests. */
+#define AB200_TILE_PAIR 0x1000
+int ab200_last_tile(void);
+
 /*
  * Limits the CTAs (= SMs) the persistent GEMM kernels launch with, process-wide; 0 restores "all".
  * Returns the previous limit.  For callers that overlap a GEMM with a collective (NCCL needs SMs of
