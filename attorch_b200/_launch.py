@@ -9,7 +9,7 @@ from typing import Optional
 import torch
 from torch.autograd import forward_ad
 
-from .linear_layer import _status_words
+from .linear_layer import _status_made, _status_words
 
 _CURRENT = contextlib.nullcontext()
 
@@ -51,11 +51,14 @@ def status_of(device: torch.device) -> int:
 
 def _new_status_word(device: torch.device) -> torch.Tensor:
     word = torch.empty(1, dtype=torch.int32, device=device)
-    if torch.cuda.is_current_stream_capturing():
-        # Recorded in the capture, the zeroing would only run with the graph's replays, and ``check_status`` before the first
-        # of them would read whatever is there.  It runs now, on a stream that is not captured.
-        with torch.cuda.stream(torch.cuda.Stream(device)):
-            word.zero_()
-    else:
+    # Recorded in a capture, the zeroing would only run with the graph's replays, and ``check_status`` before the first of
+    # them would read whatever is there: it runs now, on a stream that is not captured.
+    capturing = torch.cuda.is_current_stream_capturing()
+    stream = torch.cuda.Stream(device) if capturing else torch.cuda.current_stream(device)
+    with torch.cuda.stream(stream):
         word.zero_()
-    return _status_words.setdefault(device.index, word)          # another thread may have been first
+    made = torch.cuda.Event()
+    made.record(stream)
+    word = _status_words.setdefault(device.index, word)          # another thread may have been first
+    _status_made.setdefault(device.index, made)
+    return word

@@ -25,6 +25,7 @@ _scratch: Dict[Tuple[int, int], Dict[str, Tensor]] = {}
 _scratch_clock = 0
 # Per device index: the status word of the calls that keep no scratch (see _launch.status_of).
 _status_words: Dict[int, Tensor] = {}
+_status_made: Dict[int, torch.cuda.Event] = {}      # after the word was zeroed
 
 # Flags forwarded to every GEMM entry point (tests use them to pin a kernel family).
 _gemm_flags = 0
@@ -142,10 +143,10 @@ def check_status(device: Optional[torch.device] = None) -> None:
     words = [(key[0], entry['status']) for key, entry in list(_scratch.items())] + list(_status_words.items())
     if device is not None and device.index is not None:
         words = [(index, word) for index, word in words if index == device.index]
-    for index in {index for index, _ in words}:
-        torch.cuda.synchronize(index)               # a word is written by kernels of any stream
+    for index, made in list(_status_made.items()):
+        torch.cuda.current_stream(index).wait_event(made)
     for _, word in words:
-        code = int(word.item())
+        code = int(word.item())                     # synchronises with the current stream of the word's device
         if code != 0 and failure is None:
             word.zero_()
             failure = code

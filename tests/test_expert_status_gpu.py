@@ -65,3 +65,31 @@ def test_word_made_inside_a_capture_is_valid_at_once():
         assert torch.equal(y, torch.full_like(y, 32.0))
     finally:
         linear_layer._status_words[index] = held
+
+
+def test_check_does_not_disturb_a_capture_of_another_thread():
+    """
+    check_status reads on the current stream and waits for no stream that is being captured.  (In the capture mode that lets
+    other threads synchronise at all: the default one is ended by any read of a device value.)
+    """
+    import threading
+    x, w, offsets = captured_call()
+    errors = []
+
+    def check():
+        try:
+            attorch.check_status()
+        except Exception as error:
+            errors.append(error)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream(), capture_error_mode='thread_local'):
+        y = attorch.grouped_linear(x, offsets, w)
+        thread = threading.Thread(target=check)
+        thread.start()
+        thread.join()
+        z = attorch.grouped_linear(x, offsets, w)
+    assert not errors
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, torch.full_like(y, 32.0)) and torch.equal(y, z)
