@@ -295,12 +295,13 @@ class GateAutoGrad(torch.autograd.Function):
         ctx.needs = (input.requires_grad, weight.requires_grad)
         ctx.weight_grad_out, ctx.grad_ready, ctx.dw_chunks = weight_grad_out, grad_ready, int(dw_chunks)
         ctx.defer_input_grad = defer_input_grad
-        ctx.save_for_backward(x_op, w_op, mask)
+        # The padded rows as they are now: the caller may fill the mask's buffer for the next batch before backward.
+        ctx.save_for_backward(x_op, w_op, ~mask[:, None] if mask is not None and weight.requires_grad else None)
         return output
 
     @staticmethod
     def backward(ctx, output_grad: Tensor) -> Tuple[Optional[Tensor], ...]:
-        x_op, w_op, mask = ctx.saved_tensors
+        x_op, w_op, padded = ctx.saved_tensors
         rows, in_dim = x_op.shape
         experts, dtype, device = w_op.shape[1], x_op.dtype, x_op.device
         dt = _dtype_id(dtype)
@@ -309,8 +310,8 @@ class GateAutoGrad(torch.autograd.Function):
             # The gradient of the logits is rounded to the operands' type here, for the tensor cores.
             dy = _rows_operand(output_grad, dtype, stream_of(device))
             if ctx.needs[1]:
-                if mask is not None:
-                    x_op = _rows_operand(x_op.masked_fill(~mask[:, None], 0), dtype, stream_of(device))
+                if padded is not None:
+                    x_op = _rows_operand(x_op.masked_fill(padded, 0), dtype, stream_of(device))
                 weight_grad = ctx.weight_grad_out if ctx.weight_grad_out is not None else \
                     torch.empty((in_dim, experts), dtype=ctx.dtypes[1], device=device)
                 # Blocks of rows of dW, each handed to the gradient exchange as soon as it is enqueued.

@@ -138,3 +138,21 @@ def test_padding_may_hold_anything(gated, held, dim):
             assert torch.equal(a, b), name
     assert not results[1][0][~mask].any() and not results[1][1][~mask].any()
     attorch.check_status()
+
+
+def test_mask_buffer_can_be_reused_before_backward():
+    """Two batches in flight with one mask buffer: each backward uses what its forward was given."""
+    torch.manual_seed(6)
+    block = attorch.MixtureOfExperts(32, 48, 4, 2, 'relu', dtype=torch.bfloat16)
+    params = list(block.parameters())
+    xs = [torch.randn(60, 32, device='cuda').bfloat16() for _ in range(2)]
+    masks = [torch.rand(60, device='cuda') >= 0.3 for _ in range(2)]
+    for x, mask in zip(xs, masks):
+        x[~mask] = float('nan')
+    expected = [torch.autograd.grad(block(x, mask).float().sum(), params) for x, mask in zip(xs, masks)]
+    buffer = torch.empty(60, dtype=torch.bool, device='cuda')
+    losses = [block(x, buffer.copy_(mask)).float().sum() for x, mask in zip(xs, masks)]
+    for loss, gradients in zip(losses, expected):
+        for (name, _), a, b in zip(block.named_parameters(), torch.autograd.grad(loss, params), gradients):
+            assert torch.isfinite(a).all() and (torch.equal(a, b) or name == 'router.gate.weight'), name
+            torch.testing.assert_close(a, b, rtol=2.0 ** -7, atol=2.0 ** -7)
