@@ -131,7 +131,7 @@ __device__ __forceinline__ void place_tokens(const RouteArgs& a, int t0, int t1,
   }
 }
 
-// Turns the block's counts[warp][e] into each warp's count of what lies before it; total[e] = the block's.
+// Turns the block's counts[warp][e] into each warp's count of what lies before it; total[e] = the block's, if asked for.
 __device__ __forceinline__ void prefix_over_warps(uint16_t* counts, int experts, int* total) {
   for (int e = threadIdx.x; e < experts; e += blockDim.x) {
     int sum = 0;
@@ -141,11 +141,11 @@ __device__ __forceinline__ void prefix_over_warps(uint16_t* counts, int experts,
       counts[w * experts + e] = static_cast<uint16_t>(sum);
       sum += c;
     }
-    total[e] = sum;
+    if (total != nullptr) total[e] = sum;
   }
 }
 
-// start[e] = sum of total[0 .. e), by the first warp; returns the sum of all.
+// start[e] = sum of total[0 .. e), by one warp, lane e % 32 its e; returns the sum of all.  start may be total itself.
 __device__ __forceinline__ int scan_experts(const int* total, int experts, int lane, int* start) {
   int carry = 0;
   for (int base = 0; base < experts; base += 32) {
@@ -263,35 +263,16 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_place_kernel(const Rou
     atomicAdd(&before[e], lower);
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < E; e += blockDim.x) {
-    int sum = 0;
-#pragma unroll 8
-    for (int w = 0; w < kRouteWarps; ++w) {
-      const int c = counts[w * E + e];
-      counts[w * E + e] = static_cast<uint16_t>(sum);
-      sum += c;
-    }
-  }
+  prefix_over_warps(counts, E, nullptr);
   if (warp == 0) {
-    int carry = 0;
-    for (int base = 0; base < E; base += 32) {
-      const int e = base + lane;
-      const int c = e < E ? total[e] : 0;
-      int sum = c;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int up = __shfl_up_sync(0xFFFFFFFFu, sum, d);
-        if (lane >= d) sum += up;
-      }
-      if (e < E) {
-        before[e] += carry + sum - c;
-        if (blockIdx.x == 0) a.offsets[e] = carry + sum - c;
-      }
-      carry += __shfl_sync(0xFFFFFFFFu, sum, 31);
+    const int sum = scan_experts(total, E, lane, total);
+    for (int e = lane; e < E; e += 32) {
+      before[e] += total[e];
+      if (blockIdx.x == 0) a.offsets[e] = total[e];
     }
     if (lane == 0) {
-      *all = carry;
-      if (blockIdx.x == 0) a.offsets[E] = carry;
+      *all = sum;
+      if (blockIdx.x == 0) a.offsets[E] = sum;
     }
   }
   __syncthreads();
