@@ -267,11 +267,11 @@ class GateAutoGrad(torch.autograd.Function):
     group sums every output in one place.  The logits are fp32 whatever type is multiplied (fp32 as TF32, as in ``Linear``):
     rounded to 16 bits, near ties would become ties, which the lowest index wins.  Backward is ``Linear``'s, but rows where ``mask`` is False stay
     out of ``dW`` whatever they hold (their logits have no gradient, and zero times NaN is NaN).  The optional trailing
-    arguments are those of ``LinearAutoGrad`` for data-parallel training (where ``dW`` goes, who is told, what is put off).
+    arguments are those of ``LinearAutoGrad`` for data-parallel training: where ``dW`` goes and who is told of it.
     """
     @staticmethod
     def forward(ctx, input: Tensor, weight: Tensor, mask: Optional[Tensor] = None, weight_grad_out: Optional[Tensor] = None,
-                grad_ready=None, dw_chunks: int = 1, defer_input_grad=None) -> Tensor:
+                grad_ready=None, dw_chunks: int = 1) -> Tensor:
         assert input.ndim == 2 and input.shape[1] == weight.shape[0], \
             f'Incompatible input ({input.shape}) and weights ({weight.shape}) shape'
         assert weight.device == input.device, f'The weights are on {weight.device}, the input on {input.device}'
@@ -294,7 +294,6 @@ class GateAutoGrad(torch.autograd.Function):
         ctx.dtypes = (input.dtype, weight.dtype)
         ctx.needs = (input.requires_grad, weight.requires_grad)
         ctx.weight_grad_out, ctx.grad_ready, ctx.dw_chunks = weight_grad_out, grad_ready, int(dw_chunks)
-        ctx.defer_input_grad = defer_input_grad
         # The padded rows as they are now: the caller may fill the mask's buffer for the next batch before backward.
         ctx.save_for_backward(x_op, w_op, ~mask[:, None] if mask is not None and weight.requires_grad else None)
         return output
@@ -304,7 +303,6 @@ class GateAutoGrad(torch.autograd.Function):
         x_op, w_op, padded = ctx.saved_tensors
         rows, in_dim = x_op.shape
         experts, dtype, device = w_op.shape[1], x_op.dtype, x_op.device
-        dt = _dtype_id(dtype)
         input_grad = weight_grad = None
         with on(device):
             # The gradient of the logits is rounded to the operands' type here, for the tensor cores.
@@ -325,26 +323,13 @@ class GateAutoGrad(torch.autograd.Function):
                 ctx.grad_ready(0, 1)
             if ctx.needs[0]:
                 input_grad = torch.empty((rows, in_dim), dtype=ctx.dtypes[0], device=device)
-                address, row_bytes, dx_dtype = input_grad.data_ptr(), in_dim * input_grad.element_size(), _dtype_id(input_grad.dtype)
-
-                # Holds dY and W alive but not dX, which autograd is to be the only owner of (see LinearAutoGrad).
-                def launch_input_grad(row_begin=0, row_end=None, dz=dy, w=w_op):
-                    count = min(rows, rows if row_end is None else row_end) - row_begin
-                    if count <= 0:
-                        return
-                    with on(device):
-                        workspace, nbytes = _gemm_workspace(device, count, in_dim, experts)
-                        _lib.check(_lib.load().ab200_linear_backward_input(
-                            dz.data_ptr() + row_begin * _pitch(dz) * dz.element_size(), _ptr(w), address + row_begin * row_bytes,
-                            count, in_dim, experts, _pitch(dz), 1, _pitch(w), 1, in_dim, dt, dx_dtype, _ptr(workspace), nbytes,
-                            status_of(device), stream_of(device), _flags_for(device)), 'ab200_linear_backward_input')
-
-                if ctx.defer_input_grad is not None:
-                    ctx.defer_input_grad(launch_input_grad)
-                else:
-                    launch_input_grad()
+                workspace, nbytes = _gemm_workspace(device, rows, in_dim, experts)
+                _lib.check(_lib.load().ab200_linear_backward_input(
+                    _ptr(dy), _ptr(w_op), _ptr(input_grad), rows, in_dim, experts, _pitch(dy), 1, _pitch(w_op), 1, in_dim,
+                    _dtype_id(dtype), _dtype_id(input_grad.dtype), _ptr(workspace), nbytes, status_of(device), stream_of(device),
+                    _flags_for(device)), 'ab200_linear_backward_input')
         # A gradient that went to the caller's buffer is not returned as well: autograd would add it to ``.grad``.
-        return input_grad, None if ctx.weight_grad_out is not None else weight_grad, None, None, None, None, None
+        return input_grad, None if ctx.weight_grad_out is not None else weight_grad, None, None, None, None
 
 
 def _gemm_workspace(device: torch.device, *shape: int) -> Tuple[Optional[Tensor], int]:
@@ -389,6 +374,8 @@ class Router(nn.Module):
     def forward(self, input: Tensor, mask: Optional[Tensor] = None) -> Routing:
         """``input``: ``[tokens, dim]``; ``mask``: see ``route``."""
         gate = self.gate
-        logits = GateAutoGrad.apply(input, gate.weight, mask, gate.weight_grad_out, gate.grad_ready, gate.dw_chunks,
-                                    gate.defer_input_grad)
+        if gate.defer_input_grad is not None and input.requires_grad:
+            raise RuntimeError("The input gradient of a router's gate cannot be put off: autograd adds it to that of the dispatched "
+                               'rows. Let another layer be the first of the bucket.')
+        logits = GateAutoGrad.apply(input, gate.weight, mask, gate.weight_grad_out, gate.grad_ready, gate.dw_chunks)
         return route(logits, self.top_k, self.score_func, self.renormalize, mask)

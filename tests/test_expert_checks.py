@@ -71,3 +71,14 @@ def test_fp32_output_excludes_a_kept_pre_activation():
                                                         _lib.FLAG_OUTPUT_FP32) == -3
         assert _lib.load().ab200_grouped_linear_forward(a, a, None, None, None, a, 0, 1, 8, 8, 8, 0, 8, 8, 8, dtype, 0, 0, 0.0, a, None,
                                                         _lib.FLAG_OUTPUT_FP32) == 0
+
+
+def test_gate_refuses_to_put_its_input_gradient_off():
+    """Its input also goes to dispatch: autograd would add a gradient that has not been computed yet."""
+    from attorch_b200.dp import GradientBuckets
+    router = attorch.Router(4, 6, 2, device='cpu')
+    GradientBuckets([router.gate], defer_first_input_grad=True)
+    with pytest.raises(RuntimeError, match='put off'):
+        router(torch.zeros(3, 4, requires_grad=True))
+    with pytest.raises(RuntimeError, match='no CPU fallback'):      # nothing to put off
+        router(torch.zeros(3, 4))

@@ -42,28 +42,24 @@ def test_gate_writes_its_gradient_into_a_bucket(grad_dtype):
     attorch.check_status()
 
 
-def test_gate_tells_the_exchange_and_puts_its_input_gradient_off():
-    """Every block of dW is announced once, in order, after it has been enqueued; dX runs when the caller says so."""
+def test_gate_tells_the_exchange():
+    """Every block of dW is announced once, in order, after it has been enqueued."""
     torch.manual_seed(2)
     router = attorch.Router(64, 8, 2, 'sigmoid')
     x, dweights = torch.randn(40, 64, device='cuda'), torch.randn(40, 2, device='cuda')
     expected = gate_step(router, x, dweights)
     weight_grad = router.gate.weight.grad.clone()
     router.gate.weight.grad = None
-    told, put_off = [], []
+    told = []
     out = torch.zeros_like(router.gate.weight)
 
     def ready(block, blocks):
         told.append((block, blocks, out[block * 16:(block + 1) * 16].clone()))
 
     router.gate.weight_grad_out, router.gate.grad_ready, router.gate.dw_chunks = out, ready, 4
-    router.gate.defer_input_grad = put_off.append
     got = gate_step(router, x, dweights)
     assert [t[:2] for t in told] == [(i, 4) for i in range(4)] and router.gate.weight.grad is None
     torch.testing.assert_close(torch.cat([t[2] for t in told]), weight_grad, rtol=1e-4, atol=1e-4)
-    launch, = put_off
-    launch(0, 13)
-    launch(13)
     torch.testing.assert_close(got, expected, rtol=1e-4, atol=1e-4)
     router.gate.weight.requires_grad_(False)
     told.clear()
