@@ -156,3 +156,25 @@ def test_mask_buffer_can_be_reused_before_backward():
         for (name, _), a, b in zip(block.named_parameters(), torch.autograd.grad(loss, params), gradients):
             assert torch.isfinite(a).all() and (torch.equal(a, b) or name == 'router.gate.weight'), name
             torch.testing.assert_close(a, b, rtol=2.0 ** -7, atol=2.0 ** -7)
+
+
+@pytest.mark.parametrize('gated', [False, True])
+@pytest.mark.parametrize('shape,live', [((0, 64), 0), ((3, 0, 64), 0), ((1, 64), 1), ((1, 64), 0), ((2, 5, 64), 0), ((300, 64), 0)])
+def test_block_with_no_or_only_padded_tokens(gated, shape, live):
+    """Zero rows anywhere: outputs of the right shape, zero gradients of every parameter, none left as allocated."""
+    torch.manual_seed(7)
+    block = attorch.MixtureOfExperts(64, 96, 4, 2, 'silu', gated=gated, dtype=torch.bfloat16)
+    x = torch.randn(shape, device='cuda').bfloat16().requires_grad_()
+    mask = torch.full(shape[:-1], bool(live), device='cuda')
+    poison(4, 64, 192, dtype=x.dtype)
+    y = block(x, mask)
+    grads = torch.autograd.grad(y, [x, *block.parameters()], torch.ones_like(y))
+    assert y.shape == x.shape and grads[0].shape == x.shape
+    if live:
+        assert all(torch.isfinite(t).all() for t in (y, *grads)) and y.any() and grads[0].any()
+    else:
+        assert not y.any() and not any(t.any() for t in grads)
+    with torch.no_grad():
+        assert torch.equal(block(x, mask), y)
+        assert block.to_float8()(x, mask).shape == y.shape and (live or not block(x, mask).any())
+    attorch.check_status()
