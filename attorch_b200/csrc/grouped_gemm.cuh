@@ -21,8 +21,8 @@
 //   * Rows behind the last group (a batch with padding has fewer rows than the buffer) get zeros.
 //   * Offsets are clamped to [0, rows], made ascending and begin at 0: a bad value gives wrong rows, never a wrong
 //     address.
-// Everything else is the dense kernel's structure (gemm_tcgen05.cuh): one TMA producer
-// thread, one MMA issuer, 8 epilogue warps, two accumulators in tensor memory, optional CTA pairs.
+// Everything else is the dense kernel's structure (gemm_tcgen05.cuh): a TMA producer warp, an MMA issuer (8-bit
+// operands: two), 8 epilogue warps, two accumulators in tensor memory (8-bit: four), optional CTA pairs.
 //
 // 8-bit operands (kScaled) carry one fp32 scale per row and 128 elements of K for A and per 128 x 128
 // block for B.  A stage is exactly 128 elements of K, so each stage's product over 128 columns is one partial

@@ -174,7 +174,7 @@ def _trim_scratch() -> None:
 def _require_cuda(tensor: Tensor, what: str) -> None:
     if not tensor.is_cuda:
         raise RuntimeError(
-            f'attorch_b200.Linear runs only on CUDA devices (sm_100a); {what} is on {tensor.device}. '
+            f'attorch_b200 runs only on CUDA devices (sm_100a); {what} is on {tensor.device}. '
             'There is no CPU fallback.')
 
 
