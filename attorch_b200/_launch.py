@@ -4,6 +4,7 @@ public forms of these three took 6 of the 28 microseconds of a one-token call.
 """
 
 import contextlib
+import threading
 from typing import Optional
 
 import torch
@@ -12,6 +13,7 @@ from torch.autograd import forward_ad
 from .linear_layer import _status_made, _status_words
 
 _CURRENT = contextlib.nullcontext()
+_making = threading.Lock()
 
 
 def on(device: torch.device):
@@ -50,15 +52,17 @@ def status_of(device: torch.device) -> int:
 
 
 def _new_status_word(device: torch.device) -> torch.Tensor:
-    word = torch.empty(1, dtype=torch.int32, device=device)
-    # Recorded in a capture, the zeroing would only run with the graph's replays, and ``check_status`` before the first of
-    # them would read whatever is there: it runs now, on a stream that is not captured.
-    capturing = torch.cuda.is_current_stream_capturing()
-    stream = torch.cuda.Stream(device) if capturing else torch.cuda.current_stream(device)
-    with torch.cuda.stream(stream):
-        word.zero_()
-    made = torch.cuda.Event()
-    made.record(stream)
-    word = _status_words.setdefault(device.index, word)          # another thread may have been first
-    _status_made.setdefault(device.index, made)
+    with _making:
+        if device.index in _status_words:                        # another thread was first
+            return _status_words[device.index]
+        word = torch.empty(1, dtype=torch.int32, device=device)
+        # Recorded in a capture, the zeroing would only run with the graph's replays, and ``check_status`` before the first
+        # of them would read whatever is there: it runs now, on a stream that is not captured.
+        capturing = torch.cuda.is_current_stream_capturing()
+        stream = torch.cuda.Stream(device) if capturing else torch.cuda.current_stream(device)
+        with torch.cuda.stream(stream):
+            word.zero_()
+        _status_made[device.index] = torch.cuda.Event()
+        _status_made[device.index].record(stream)
+        _status_words[device.index] = word
     return word

@@ -265,9 +265,9 @@ class GateAutoGrad(torch.autograd.Function):
     reduction of a product this narrow out over all SMs and adds the pieces atomically, in an order that changes
     from call to call; a token whose logits nearly tie could then change its experts.  The grouped kernel with one
     group sums every output in one place.  The logits are fp32 whatever type is multiplied (fp32 as TF32, as in ``Linear``):
-    rounded to 16 bits, near ties would become ties, which the lowest index wins.  Backward is ``Linear``'s, but rows where ``mask`` is False stay
-    out of ``dW`` whatever they hold (their logits have no gradient, and zero times NaN is NaN).  The optional trailing
-    arguments are those of ``LinearAutoGrad`` for data-parallel training: where ``dW`` goes and who is told of it.
+    rounded to 16 bits, near ties would become ties, which the lowest index wins.  Backward is ``Linear``'s, but rows where
+    ``mask`` is False stay out of ``dW`` whatever they hold (their logits have no gradient, and zero times NaN is NaN).  The
+    optional trailing arguments are those of ``LinearAutoGrad`` for data-parallel training: where ``dW`` goes and who is told of it.
     """
     @staticmethod
     def forward(ctx, input: Tensor, weight: Tensor, mask: Optional[Tensor] = None, weight_grad_out: Optional[Tensor] = None,
@@ -377,5 +377,6 @@ class Router(nn.Module):
         if gate.defer_input_grad is not None and input.requires_grad:
             raise RuntimeError("The input gradient of a router's gate cannot be put off: autograd adds it to that of the dispatched "
                                'rows. Let another layer be the first of the bucket.')
-        logits = GateAutoGrad.apply(input, gate.weight, mask, gate.weight_grad_out, gate.grad_ready, gate.dw_chunks)
+        padding = mask if torch.is_grad_enabled() else None          # the gate needs it for its gradient only
+        logits = GateAutoGrad.apply(input, gate.weight, padding, gate.weight_grad_out, gate.grad_ready, gate.dw_chunks)
         return route(logits, self.top_k, self.score_func, self.renormalize, mask)

@@ -93,3 +93,27 @@ def test_check_does_not_disturb_a_capture_of_another_thread():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(y, torch.full_like(y, 32.0)) and torch.equal(y, z)
+
+
+def test_threads_that_come_first_together_share_one_word():
+    import threading
+    x, w, offsets = captured_call()
+    index = x.device.index
+    held = linear_layer._status_words.pop(index)
+    seen, start = [], threading.Barrier(8)
+
+    def call():
+        start.wait()
+        attorch.grouped_linear(x, offsets, w)
+        seen.append(status_of(x.device))
+
+    try:
+        threads = [threading.Thread(target=call) for _ in range(8)]
+        for thread in threads:
+            thread.start()
+        for thread in threads:
+            thread.join()
+        assert len(seen) == 8 and set(seen) == {linear_layer._status_words[index].data_ptr()}
+        attorch.check_status()
+    finally:
+        linear_layer._status_words[index] = held
